@@ -14,7 +14,9 @@ SOURCES = ['engine.hip', 'mfma_kernels.hip', 'chain_kernels.hip', 'cached_kernel
            'cached_kernels_c.hip']
 HEADERS = sorted(f for f in os.listdir(CSRC) if f.endswith('.h')) + [os.path.join('..', '..', 'include', 'muzero_amd.h')]
 # -ffp-contract=off: the tree arithmetic must round exactly like the reference's NumPy expressions.
-FLAGS = ['--offload-arch=gfx950', '-ffp-contract=off', '-fPIC', '-std=c++17']
+# No packed float32 instructions (v_pk_add / mul / fma_f32): some of their forms have returned wrong values now and then.
+FLAGS = ['--offload-arch=gfx950', '-ffp-contract=off', '-fPIC', '-std=c++17',
+         '-Xclang', '-target-feature', '-Xclang', '-packed-fp32-ops']
 # Optimisation level per translation unit, as measured (same box, both builds): the whole-search kernels of the matrix-core
 # units are larger than the 64 KB instruction cache, and optimising for size makes them 0.7 - 0.9 % faster (TicTacToe
 # 16384 x 100: 7.15 -> 7.10 ms, Atari-shaped 1024 x 200: 7.84 -> 7.78 ms); the register-resident tree kernels of
