@@ -407,6 +407,96 @@ int mz_legacy_root_noise(uint32_t *mt_key, int32_t *mt_pos, double alpha, int32_
  * order; state in and out as for mz_legacy_root_noise.  Host only; the logarithms run on a few host threads. */
 int mz_legacy_gumbel(uint32_t *mt_key, int32_t *mt_pos, int64_t n, double *out);
 
+/* ---- Tensor operators around a policy that learns from the search and plays ahead of it.  No context: device pointers,
+ * HOST argument structs, work enqueued on `stream` of the current device; no allocation, no synchronisation. */
+
+/* Element types. */
+#define MZ_F32 0
+#define MZ_BF16 1
+#define MZ_F16 2
+#define MZ_F64 3
+
+/* A [B][T][D] tensor: element (b, t, d) at p + b * stride_b + t * stride_t + d * stride_d (in elements, any sign, zero
+ * for a broadcast axis of an input). */
+typedef struct mz_strided {
+    void *p;
+    int64_t stride_b, stride_t, stride_d;
+} mz_strided;
+
+/* Gated linear recurrence along T, out[t] = gate[t] * out[t-1] + x[t] (reverse: out[t] = gate[t] * out[t+1] + x[t]), the
+ * sum behind discounted returns and traces (games/game.py:205-236 sums one of them term by term).  All tensors of one
+ * element type; states [B][D] contiguous, float32 (float64 for MZ_F64), as is the arithmetic: one rounding per output.
+ * Runs of positions are composed through products of their gates, which must not overflow (|gate| <= 1 cannot).
+ * mz_linear_recurrence: gate, x -> out; state = what precedes the first position (NULL: 0), last = the state behind the
+ * last position (may be NULL).
+ * mz_linear_recurrence_backward: gate as before, x = gradient of out -> out = gradient of x; with y = the outputs,
+ * out_gate = gradient of gate (both or neither; state as before); grad_last = gradient of last (NULL: 0), out_state =
+ * gradient of state (may be NULL).  Inputs and outputs must not overlap. */
+typedef struct mz_recurrence {
+    int32_t type, B, D, reverse;
+    int64_t T;
+    mz_strided gate, x, out, y, out_gate;
+    const void *state;
+    void *last;
+    const void *grad_last;
+    void *out_state;
+} mz_recurrence;
+int mz_linear_recurrence(const mz_recurrence *args_h, void *stream);
+int mz_linear_recurrence_backward(const mz_recurrence *args_h, void *stream);
+
+/* Distillation of a policy from a teacher's top logits: loss[r] = weight[r] * temperature^2 * KL(p || q), q =
+ * softmax(logits / temperature) over the V actions; p = softmax(teacher / temperature) over the K entries, or, with lse
+ * (log-sum-exp of the teacher's logits / temperature over all actions), p = exp(teacher / temperature - lse) and one more
+ * class of all actions outside the entries (left out where the student gives those nothing).  The soft cross-entropy the
+ * trainer takes over whole rows (trainer.py:119-122), for targets that name few actions.
+ * Entries whose index lies outside 0..V-1 are absent; an action named twice gets the sum.  Rows without entries and
+ * rows of weight 0 have loss and gradient 0 whatever their logits hold.
+ * mz_distill_loss: loss and stats.  mz_distill_grad: grad = grad_loss[r] * d loss[r] / d logits from those stats.
+ * mz_distill_loss_grad: loss and grad (grad_loss taken as 1) with the logits read once. */
+#define MZ_DISTILL_MAX_ENTRIES 1024
+#define MZ_DISTILL_MAX_TAIL_ACTIONS 262144
+typedef struct mz_distill {
+    int32_t type, teacher_type, index64;   /* MZ_F32 / MZ_BF16 / MZ_F16; 1 = index is int64, 0 = int32 */
+    int32_t R, V, K;
+    float temperature;
+    const void *logits;      /* [R][V], rows logits_stride elements apart */
+    int64_t logits_stride;
+    const void *index;       /* [R][K] */
+    const void *teacher;     /* [R][K] */
+    const float *lse;        /* [R] or NULL */
+    const float *weight;     /* [R] or NULL: 1 */
+    const float *grad_loss;  /* [R] or NULL: 1 */
+    float *loss;             /* [R] */
+    void *grad;              /* [R][V], type of logits; must not overlap the logits */
+    float *stats;            /* [R][4] */
+} mz_distill;
+int mz_distill_loss(const mz_distill *args_h, void *stream);
+int mz_distill_grad(const mz_distill *args_h, void *stream);
+int mz_distill_loss_grad(const mz_distill *args_h, void *stream);
+
+/* Verification of drafted moves: of sequence b's drafts x_0 .. x_(length-1), played by the policy `draft`, the first are
+ * kept while u_accept[k] * draft_k(x_k) < target_k(x_k); the first that is not is replaced by a token drawn from
+ * max(target_k - draft_k, 0) (from target_k where that is nowhere positive), and where all are kept one more is drawn from
+ * the target's next row, so that what is played is distributed as the target's own moves (the rule that draws one,
+ * mcts/action_selection.py:69).  A draw is the first index whose running sum exceeds u_sample[b] * the whole, in float64.
+ * Entries that are negative, infinite or NaN count as 0; a drafted token outside 0..V-1 is not kept; a target row without
+ * any mass yields token -1.  out holds the kept drafts, the drawn token, and -1 behind it. */
+typedef struct mz_verify {
+    int32_t type, token64;      /* type of draft and target; 1 = tokens and out are int64, 0 = int32 */
+    int32_t B, K, V, reserved;
+    const void *tokens;         /* [B][K] */
+    const void *draft;          /* [B][K][V], V contiguous; NULL: each draft was its policy's only choice */
+    int64_t draft_stride_b, draft_stride_k;
+    const void *target;         /* [B][K + 1][V], V contiguous */
+    int64_t target_stride_b, target_stride_k;
+    const double *u_accept;     /* [B][K], uniform in [0, 1) */
+    const double *u_sample;     /* [B] */
+    const int32_t *lengths;     /* [B], clamped to 0..K, or NULL: K */
+    int32_t *accepted;          /* [B] */
+    void *out;                  /* [B][K + 1] */
+} mz_verify;
+int mz_verify_drafts(const mz_verify *args_h, void *stream);
+
 /* Library/ABI version. */
 int mz_version(void);
 

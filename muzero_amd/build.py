@@ -9,9 +9,9 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, 'csrc')
 LIB = os.path.join(HERE, 'libmuzero_amd.so')
 OBJ_DIR = os.path.join(HERE, 'build')
-# translation units: the C ABI with the tree / fused-network kernels, and the matrix-core kernels
+# translation units: the C ABI with the tree / fused-network kernels, the matrix-core kernels, and the tensor operators
 SOURCES = ['engine.hip', 'mfma_kernels.hip', 'chain_kernels.hip', 'cached_kernels_a.hip', 'cached_kernels_b.hip',
-           'cached_kernels_c.hip']
+           'cached_kernels_c.hip', 'policy_kernels.hip']
 HEADERS = sorted(f for f in os.listdir(CSRC) if f.endswith('.h')) + [os.path.join('..', '..', 'include', 'muzero_amd.h')]
 # -ffp-contract=off: the tree arithmetic must round exactly like the reference's NumPy expressions.
 # No packed float32 instructions (v_pk_add / mul / fma_f32): some of their forms have returned wrong values now and then.
@@ -26,7 +26,7 @@ FLAGS = ['--offload-arch=gfx950', '-ffp-contract=off', '-fPIC', '-std=c++17',
 # mfma_kernels.hip lose 1.6 - 2.7 % under each of the three and keep the default scheduler.
 _CACHED = '-Os -mllvm --amdgpu-sched-strategy=iterative-ilp'
 OPT = {'engine.hip': '-O3', 'chain_kernels.hip': '-O3', 'cached_kernels_a.hip': _CACHED, 'cached_kernels_b.hip': _CACHED,
-       'cached_kernels_c.hip': _CACHED}
+       'cached_kernels_c.hip': _CACHED, 'policy_kernels.hip': '-O3'}
 OPT_DEFAULT = '-Os'
 
 
@@ -52,8 +52,10 @@ def needs_build(lib: str = LIB) -> bool:
 
 
 # headers a translation unit does NOT include (everything else counts as a dependency)
-_TREE_ONLY = {'search_net.h', 'search_reg.h', 'env_step.h', 'targets.h'}
-NOT_INCLUDED = {'engine.hip': {'net_mfma.h', 'search_cached.h', 'search_chain.h', 'cached_launch.h'},
+_POLICY = {'element_types.h', 'recurrence.h', 'distill.h', 'verify.h'}
+_TREE_ONLY = {'search_net.h', 'search_reg.h', 'env_step.h', 'targets.h', 'api.h'} | _POLICY
+NOT_INCLUDED = {'engine.hip': {'net_mfma.h', 'search_cached.h', 'search_chain.h', 'cached_launch.h'} | _POLICY,
+                'policy_kernels.hip': {os.path.basename(h) for h in HEADERS} - _POLICY - {'api.h', 'muzero_amd.h'},
                 'mfma_kernels.hip': _TREE_ONLY | {'search_chain.h', 'cached_launch.h'},
                 'chain_kernels.hip': _TREE_ONLY | {'search_cached.h', 'cached_launch.h'},
                 'cached_kernels_a.hip': _TREE_ONLY | {'search_chain.h'},

@@ -20,6 +20,7 @@
 #include <mutex>
 #include <utility>
 #include "../../include/muzero_amd.h"
+#include "api.h"
 #include "tree_kernels.h"  // device_common.h, tree_ops.h
 #include "dense_net.h"
 #include "mfma_launch.h"   // matrix-core leaf evaluation and searches, compiled in mfma_kernels.hip
@@ -547,6 +548,9 @@ static int launch_status(const char *fn)
     if (e != hipSuccess) return fail(MZ_ERR_HIP, std::string(fn) + ": launch failed: " + hipGetErrorString(e));
     return MZ_OK;
 }
+
+int mz::api_fail(int code, const std::string &msg) { return fail(code, msg); }
+int mz::api_launch_status(const char *fn) { return launch_status(fn); }
 
 extern "C" int mz_root_prepare(mz_ctx *c, int32_t B, const float *logits, const double *dirichlet,
                                double frac, const uint8_t *legal, int32_t shift_and_mask, void *out_prior,

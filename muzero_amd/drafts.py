@@ -1,0 +1,67 @@
+"""Playing ahead of the search: moves drafted by a cheap policy, verified against the search's own.
+
+A cheap policy (a distilled network, or the raw prior) plays several moves ahead; one batched search then evaluates all the
+positions it passed through, and `verify_drafts` keeps the drafted moves as far as they are distributed like the search's:
+the moves that come out follow the search's policies exactly (mcts/action_selection.py:56-72 is the rule that draws one)."""
+from __future__ import annotations
+
+from typing import Optional, Tuple
+
+import torch
+
+from . import engine as _engine
+
+
+def verify_drafts(tokens: torch.Tensor, draft: Optional[torch.Tensor], target: torch.Tensor, u_accept: torch.Tensor,
+                  u_sample: torch.Tensor, lengths: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Keeps drafted move k of a sequence while u_accept[k] * draft[k, x_k] < target[k, x_k]; replaces the first that is not
+    kept by a draw from max(target[k] - draft[k], 0) (from target[k] where that is nowhere positive); where all are kept,
+    draws one more from the target's next row.
+
+    tokens [B, K] int32 / int64; draft [B, K, V] the probabilities they were drawn from, or None where each was its policy's
+    only choice; target [B, K + 1, V] of the same type (float64, float32, bfloat16, float16); u_accept [B, K] and u_sample
+    [B] float64 uniforms of [0, 1); lengths int32 [B]: drafted moves of each sequence (None: K).  Sums are float64 and a draw
+    takes the first index whose running sum exceeds u * the whole, as np.random.choice does.  Probabilities that are
+    negative, infinite or NaN count as 0, a drafted move outside 0..V-1 is not kept.
+    Returns (accepted int32 [B], moves [B, K + 1] of the type of tokens: the kept drafts, the drawn move, -1 behind it; a
+    target row without any mass yields -1)."""
+    named = (('tokens', tokens), ('draft', draft), ('target', target), ('u_accept', u_accept), ('u_sample', u_sample), ('lengths', lengths))
+    for name, t in named:
+        if t is None and name in ('draft', 'lengths'):
+            continue
+        if not torch.is_tensor(t) or not t.is_cuda:
+            raise _engine.EngineError(f'verify_drafts needs device tensors (there is no CPU fallback): {name}')
+        if t.device != target.device:
+            raise ValueError(f'verify_drafts: {name} is on another device than the target')
+    if tokens.dim() != 2 or target.dim() != 3:
+        raise ValueError('verify_drafts: tokens [B, K] and target [B, K + 1, V] expected')
+    B, K = tokens.shape
+    V = target.shape[2]
+    if tuple(target.shape) != (B, K + 1, V) or (draft is not None and tuple(draft.shape) != (B, K, V)) or V < 1:
+        raise ValueError(f'verify_drafts: target must be [B, K + 1, V] and draft [B, K, V], got {tuple(target.shape)} and '
+                         f'{None if draft is None else tuple(draft.shape)} for {B} x {K} tokens')
+    if target.dtype not in _engine.ELEMENT_TYPES or (draft is not None and draft.dtype != target.dtype):
+        raise ValueError('verify_drafts: draft and target must share a floating type')
+    if tokens.dtype not in (torch.int32, torch.int64):
+        raise ValueError('verify_drafts: tokens must be int32 or int64')
+    if tuple(u_accept.shape) != (B, K) or tuple(u_sample.shape) != (B,) or u_accept.dtype != torch.float64 or u_sample.dtype != torch.float64:
+        raise ValueError('verify_drafts: u_accept [B, K] and u_sample [B] must be float64')
+    if lengths is not None and (tuple(lengths.shape) != (B,) or lengths.dtype != torch.int32):
+        raise ValueError('verify_drafts: lengths must be int32 [B]')
+    accepted = torch.empty(B, dtype=torch.int32, device=target.device)
+    out = torch.empty((B, K + 1), dtype=tokens.dtype, device=target.device)
+    if B == 0:
+        return accepted, out
+    if target.stride(2) != 1 and V > 1:
+        target = target.contiguous()
+    if draft is not None and draft.stride(2) != 1 and V > 1:
+        draft = draft.contiguous()
+    tokens, u_accept, u_sample = tokens.contiguous(), u_accept.contiguous(), u_sample.contiguous()
+    lengths = None if lengths is None else lengths.contiguous()
+    p = lambda t: None if t is None else t.data_ptr()  # noqa: E731
+    sd = (0, 0) if draft is None else draft.stride()[:2]
+    args = _engine.MzVerify(_engine.ELEMENT_TYPES[target.dtype], int(tokens.dtype == torch.int64), B, K, V, 0, p(tokens), p(draft),
+                            *sd, p(target), target.stride(0), target.stride(1), p(u_accept), p(u_sample), p(lengths),
+                            p(accepted), p(out))
+    _engine.launch_on(target.device, _engine.lib().mz_verify_drafts, args, 'mz_verify_drafts')
+    return accepted, out

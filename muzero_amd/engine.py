@@ -53,12 +53,40 @@ class MzMoveLog(C.Structure):
                 ('root_values', C.c_void_p), ('probs', C.c_void_p), ('done', C.c_void_p), ('open_at_start', C.c_void_p)]
 
 
+class MzStrided(C.Structure):
+    _fields_ = [('p', C.c_void_p), ('stride_b', C.c_int64), ('stride_t', C.c_int64), ('stride_d', C.c_int64)]
+
+
+class MzRecurrence(C.Structure):
+    _fields_ = [('type', C.c_int32), ('B', C.c_int32), ('D', C.c_int32), ('reverse', C.c_int32), ('T', C.c_int64),
+                ('gate', MzStrided), ('x', MzStrided), ('out', MzStrided), ('y', MzStrided), ('out_gate', MzStrided),
+                ('state', C.c_void_p), ('last', C.c_void_p), ('grad_last', C.c_void_p), ('out_state', C.c_void_p)]
+
+
+class MzDistill(C.Structure):
+    _fields_ = [('type', C.c_int32), ('teacher_type', C.c_int32), ('index64', C.c_int32), ('R', C.c_int32), ('V', C.c_int32),
+                ('K', C.c_int32), ('temperature', C.c_float), ('logits', C.c_void_p), ('logits_stride', C.c_int64),
+                ('index', C.c_void_p), ('teacher', C.c_void_p), ('lse', C.c_void_p), ('weight', C.c_void_p),
+                ('grad_loss', C.c_void_p), ('loss', C.c_void_p), ('grad', C.c_void_p), ('stats', C.c_void_p)]
+
+
+class MzVerify(C.Structure):
+    _fields_ = [('type', C.c_int32), ('token64', C.c_int32), ('B', C.c_int32), ('K', C.c_int32), ('V', C.c_int32),
+                ('reserved', C.c_int32), ('tokens', C.c_void_p), ('draft', C.c_void_p), ('draft_stride_b', C.c_int64),
+                ('draft_stride_k', C.c_int64), ('target', C.c_void_p), ('target_stride_b', C.c_int64),
+                ('target_stride_k', C.c_int64), ('u_accept', C.c_void_p), ('u_sample', C.c_void_p), ('lengths', C.c_void_p),
+                ('accepted', C.c_void_p), ('out', C.c_void_p)]
+
+
 ENV_TICTACTOE, ENV_CARTPOLE = 1, 2
+# element types of the tensor operators (MZ_F32 ...)
+ELEMENT_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2, torch.float64: 3}
 
 EXPORTS = ['mz_create', 'mz_destroy', 'mz_last_error', 'mz_set_seed', 'mz_check', 'mz_root_prepare', 'mz_tree_reset', 'mz_select',
            'mz_select_outputs', 'mz_expand_backup', 'mz_to_act', 'mz_search_run', 'mz_search_run_act', 'mz_search_move', 'mz_set_network', 'mz_set_root_network', 'mz_search_begin_net', 'mz_set_network_mfma', 'mz_set_root_network_mfma', 'mz_initial_inference_mfma', 'mz_expand_backup_net', 'mz_expand_backup_net_static', 'mz_act_env_step', 'mz_act_env_step_log', 'mz_log_count_games', 'mz_log_list_games', 'mz_tree_export',
            'mz_stats', 'mz_node_qtransform', 'mz_node_select', 'mz_node_backward', 'mz_tree_import', 'mz_considered_visits', 'mz_legacy_root_noise', 'mz_legacy_gumbel', 'mz_make_targets', 'mz_scalar_to_support',
-           'mz_version']
+           'mz_linear_recurrence', 'mz_linear_recurrence_backward', 'mz_distill_loss', 'mz_distill_grad',
+           'mz_distill_loss_grad', 'mz_verify_drafts', 'mz_version']
 
 
 def lib():
@@ -108,6 +136,10 @@ def lib():
         L.mz_node_qtransform.argtypes = [vp, i32, i32, i32, vp, vp]
         L.mz_node_select.argtypes = [vp, i32, i32, i32, vp, vp, vp]
         L.mz_considered_visits.argtypes = [i32, i32, vp]
+        for name, struct in (('mz_linear_recurrence', MzRecurrence), ('mz_linear_recurrence_backward', MzRecurrence),
+                             ('mz_distill_loss', MzDistill), ('mz_distill_grad', MzDistill),
+                             ('mz_distill_loss_grad', MzDistill), ('mz_verify_drafts', MzVerify)):
+            getattr(L, name).argtypes = [C.POINTER(struct), vp]
         _lib = L
     return _lib
 
@@ -194,6 +226,15 @@ def _stream():
     if raw is not None:
         return C.c_void_p(raw(torch.cuda.current_device()))
     return C.c_void_p(torch.cuda.current_stream().cuda_stream)
+
+
+def launch_on(device, fn, struct, what):
+    """Calls a tensor operator's entry point on the current stream of `device`, which need not be the current one."""
+    if device.index == torch.cuda.current_device():
+        _check(fn(C.byref(struct), _stream()), what)
+    else:
+        with torch.cuda.device(device):
+            _check(fn(C.byref(struct), _stream()), what)
 
 
 class SearchEngine:

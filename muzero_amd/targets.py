@@ -9,7 +9,7 @@ padding, `GameHistory.make_target`) runs as one kernel over all sampled position
 from __future__ import annotations
 
 import ctypes as C
-from typing import List, Sequence
+from typing import List, Optional, Sequence
 
 import numpy as np
 import torch
@@ -67,6 +67,28 @@ class MoveLog:
         return base, length
 
 
+    def lambda_returns(self, gamma: float, lam: float, bootstrap=None) -> torch.Tensor:
+        """Lambda returns of every position in the written rows, float64 [rows, B] in the view of the player to move:
+        G[t] = r[t] + gamma * s * ((1 - lam) * v[t+1] + lam * G[t+1]), cut behind the last move of a game; v are the
+        recorded root values and s is -1 where the mover changes, else 1.  lam = 1 is the whole discounted return.
+        bootstrap [B]: value behind the last row in the view of that row's mover, for games that are still open (None: 0)."""
+        n = self.rows
+        if n < 1:
+            raise ValueError('lambda_returns: the log holds no move')
+        rewards, values, players = self.rewards[:n], self.root_values[:n], self.to_plays[:n]
+        after = torch.zeros_like(values)
+        after[:-1] = values[1:]
+        sign = torch.ones_like(values)
+        sign[:-1] = torch.where(players[1:] == players[:-1], 1.0, -1.0)
+        if bootstrap is not None:
+            after[-1] = torch.as_tensor(bootstrap, dtype=torch.float64, device=self.device).reshape(self.B)
+        onward = float(gamma) * sign * (self.done[:n] == 0)
+        weight = torch.full((n, 1), 1.0 - float(lam), dtype=torch.float64, device=self.device)
+        weight[-1] = 1.0                                   # nothing follows the last row but its bootstrap value
+        y, _ = linear_recurrence((onward * float(lam))[None], (rewards + onward * weight * after)[None], reverse=True)
+        return y[0]
+
+
 def scalar_to_support(x: torch.Tensor, support_limit: int) -> torch.Tensor:
     """Categorical form of value / reward targets, as the trainer builds it (trainer.py:70-71 ->
     utils/network_utils.py:99-129): float32 device tensor (...,) -> (..., 2 * support_limit + 1)."""
@@ -77,6 +99,124 @@ def scalar_to_support(x: torch.Tensor, support_limit: int) -> torch.Tensor:
     _check(lib().mz_scalar_to_support(_ptr(xf), C.c_int64(xf.numel()), C.c_int32(int(support_limit)), _ptr(out), _stream()),
            'mz_scalar_to_support')
     return out
+
+
+_STATE_TYPE = {torch.float64: torch.float64}
+
+
+def _strided(t) -> '_engine.MzStrided':
+    return _engine.MzStrided(t.data_ptr(), *t.stride())
+
+
+def _lined_up(t: torch.Tensor, channels: bool) -> torch.Tensor:
+    """`t` itself where the kernels read its layout well: channels contiguous, or (one channel, or time contiguous) any."""
+    return t.contiguous() if channels and t.stride(2) != 1 else t
+
+
+def _like(x: torch.Tensor, channels: bool) -> torch.Tensor:
+    y = torch.empty_like(x)
+    return torch.empty(x.shape, dtype=x.dtype, device=x.device) if channels and y.stride(2) != 1 else y
+
+
+def _recurrence_call(backward, gate, x, state, reverse, out, last=None, y=None, out_gate=None, grad_last=None, out_state=None):
+    views = [gate, x, out, y, out_gate]
+    B, T, D = x.shape
+    if D == 1 and T > 1 and x.stride(1) != 1 and x.stride(0) == 1:
+        # one channel, time-major: the rows are the channels of a single sequence
+        views = [None if v is None else v.transpose(0, 2) for v in views]
+        if any(v is not None and v.stride(2) != 1 for v in views):
+            views = [gate, x, out, y, out_gate]
+        else:
+            B, D = 1, B
+    none = _engine.MzStrided()
+    p = lambda t: None if t is None else t.data_ptr()  # noqa: E731
+    args = _engine.MzRecurrence(_engine.ELEMENT_TYPES[x.dtype], B, D, int(reverse), T,
+                                *[none if v is None else _strided(v) for v in views], p(state), p(last), p(grad_last), p(out_state))
+    L = lib()
+    if backward:
+        _engine.launch_on(x.device, L.mz_linear_recurrence_backward, args, 'mz_linear_recurrence_backward')
+    else:
+        _engine.launch_on(x.device, L.mz_linear_recurrence, args, 'mz_linear_recurrence')
+
+
+def _recurrence_forward(gate, x, state, reverse):
+    B, T, D = x.shape
+    wide = _STATE_TYPE.get(x.dtype, torch.float32)
+    if x.numel() == 0:
+        last = torch.zeros((B, D), dtype=wide, device=x.device) if state is None else state.clone()
+        return torch.empty_like(x), last
+    channels = D > 1 and (x.stride(2) == 1 or x.stride(1) != 1)
+    gate, x = _lined_up(gate, channels), _lined_up(x, channels)
+    y = _like(x, channels)
+    last = torch.empty((B, D), dtype=wide, device=x.device)
+    _recurrence_call(False, gate, x, state, reverse, y, last)
+    return y, last
+
+
+class _LinearRecurrence(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, gate, x, state, reverse):
+        y, last = _recurrence_forward(gate, x, state, reverse)
+        ctx.reverse = reverse
+        ctx.set_materialize_grads(False)
+        ctx.save_for_backward(gate, y if gate.requires_grad else None, state)
+        ctx.like = (x.shape, x.dtype, x.device)
+        return y, last
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy, dlast):
+        gate, y, state = ctx.saved_tensors
+        shape, dtype, device = ctx.like
+        want_gate, want_x, want_state, _ = ctx.needs_input_grad
+        if dy is None and dlast is None:
+            return None, None, None, None
+        if dy is None:
+            dy = torch.zeros(shape, dtype=dtype, device=device)
+        wide = _STATE_TYPE.get(dtype, torch.float32)
+        dstate = torch.empty((shape[0], shape[2]), dtype=wide, device=device) if want_state else None
+        if dlast is not None:
+            dlast = dlast.contiguous()
+        if dy.numel() == 0:
+            return (torch.empty(shape, dtype=dtype, device=device) if want_gate else None,
+                    torch.empty(shape, dtype=dtype, device=device) if want_x else None,
+                    (torch.zeros_like(dstate) if dlast is None else dlast.clone()) if want_state else None, None)
+        channels = shape[2] > 1 and (dy.stride(2) == 1 or dy.stride(1) != 1)
+        gate, dy = _lined_up(gate, channels), _lined_up(dy, channels)
+        dx = _like(dy, channels)
+        dgate = None
+        if want_gate:
+            y, dgate = _lined_up(y, channels), _like(dy, channels)
+        _recurrence_call(True, gate, dy, state, ctx.reverse, dx, y=y if want_gate else None, out_gate=dgate, grad_last=dlast,
+                         out_state=dstate)
+        return dgate, dx if want_x else None, dstate, None
+
+
+def linear_recurrence(gate: torch.Tensor, x: torch.Tensor, state: Optional[torch.Tensor] = None, reverse: bool = False):
+    """y[:, t] = gate[:, t] * y[:, t-1] + x[:, t] along axis 1 of device tensors [B, T, D] (`reverse`: from the last
+    position to the first, the direction of returns), differentiable in gate, x and state.
+
+    gate and x share shape and type (float32, bfloat16, float16, float64); any strides are read, those with contiguous
+    channels or contiguous time without a copy, and a gate may be expanded along any axis.  state [B, D]: what precedes the
+    first position, float32 (float64 with float64 tensors) - zeros if None.  Returns (y, state behind the last position);
+    that state continues the recurrence in a later call, one position at a time if need be.  Arithmetic is float32 (float64
+    for float64), each y rounded once.  The products of the gates over a record must not overflow, which |gate| <= 1
+    ensures; a gate of 0 cuts the record."""
+    if not (torch.is_tensor(gate) and torch.is_tensor(x) and gate.is_cuda and x.is_cuda):
+        raise _engine.EngineError('linear_recurrence needs device tensors (there is no CPU fallback)')
+    if x.dim() != 3 or gate.shape != x.shape:
+        raise ValueError(f'linear_recurrence: gate and x must both be [B, T, D], got {tuple(gate.shape)} and {tuple(x.shape)}')
+    if x.dtype not in _engine.ELEMENT_TYPES or gate.dtype != x.dtype:
+        raise ValueError(f'linear_recurrence: gate and x must share a floating type, got {gate.dtype} and {x.dtype}')
+    if gate.device != x.device:
+        raise ValueError('linear_recurrence: gate and x are on different devices')
+    if state is not None:
+        if state.shape != (x.shape[0], x.shape[2]) or state.dtype != _STATE_TYPE.get(x.dtype, torch.float32) or state.device != x.device:
+            raise ValueError(f'linear_recurrence: state must be {_STATE_TYPE.get(x.dtype, torch.float32)} [B, D] on the device of x')
+        state = state.contiguous()
+    if torch.is_grad_enabled() and (gate.requires_grad or x.requires_grad or (state is not None and state.requires_grad)):
+        return _LinearRecurrence.apply(gate, x, state, bool(reverse))
+    return _recurrence_forward(gate, x, state, bool(reverse))
 
 
 class TrajectoryStore:

@@ -19,12 +19,13 @@ unweighted; loss = (value_loss_weight * value + reward + policy) / 3 (trainer.py
 """
 from __future__ import annotations
 
-from typing import Tuple
+from typing import Optional, Tuple
 
 import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
+from . import engine as _engine
 from .targets import scalar_to_support
 
 
@@ -46,6 +47,92 @@ def soft_cross_entropy(logits: torch.Tensor, target: torch.Tensor) -> torch.Tens
     """Cross-entropy against probability targets, averaged over the batch axis: `[..., B, C]` -> `[...]`
     (what `nn.CrossEntropyLoss()` computes for one `[B, C]` slice, trainer.py:119-122)."""
     return -(target * F.log_softmax(logits, dim=-1)).sum(dim=-1).mean(dim=-1)
+
+
+def _distill_args(logits, index, teacher, teacher_lse, temperature, weight):
+    """Checks the arguments of the distillation calls; returns (MzDistill without outputs, tensors it points to)."""
+    for name, t in (('logits', logits), ('index', index), ('teacher', teacher), ('teacher_lse', teacher_lse), ('weight', weight)):
+        if t is None and name in ('teacher_lse', 'weight'):
+            continue
+        if not torch.is_tensor(t) or not t.is_cuda:
+            raise _engine.EngineError(f'distillation needs device tensors (there is no CPU fallback): {name}')
+        if t.device != logits.device:
+            raise ValueError(f'distillation: {name} is on another device than the logits')
+    if logits.dim() != 2 or index.dim() != 2 or index.shape[0] != logits.shape[0] or teacher.shape != index.shape:
+        raise ValueError(f'distillation: logits [R, V], index and teacher [R, K] expected, got {tuple(logits.shape)}, '
+                         f'{tuple(index.shape)}, {tuple(teacher.shape)}')
+    types = _engine.ELEMENT_TYPES
+    if types.get(logits.dtype, 3) == 3 or types.get(teacher.dtype, 3) == 3 or index.dtype not in (torch.int32, torch.int64):
+        raise ValueError('distillation: logits and teacher are float32, bfloat16 or float16, index is int32 or int64')
+    R, V = logits.shape
+    K = index.shape[1]
+    for name, t in (('teacher_lse', teacher_lse), ('weight', weight)):
+        if t is not None and (t.shape != (R,) or t.dtype != torch.float32):
+            raise ValueError(f'distillation: {name} must be float32 [{R}]')
+    if logits.stride(1) != 1 or logits.stride(0) < 0:
+        logits = logits.contiguous()
+    logits, index, teacher = logits.detach(), index.contiguous(), teacher.detach().contiguous()
+    lse = None if teacher_lse is None else teacher_lse.detach().contiguous()
+    weight = None if weight is None else weight.detach().contiguous()
+    p = lambda t: None if t is None else t.data_ptr()  # noqa: E731
+    args = _engine.MzDistill(types[logits.dtype], types[teacher.dtype], int(index.dtype == torch.int64), R, V, K,
+                             float(temperature), p(logits), logits.stride(0), p(index), p(teacher), p(lse), p(weight))
+    return args, (logits, index, teacher, lse, weight)
+
+
+class _Distillation(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, index, teacher, teacher_lse, temperature, weight):
+        args, kept = _distill_args(logits, index, teacher, teacher_lse, temperature, weight)
+        R = logits.shape[0]
+        loss = torch.empty(R, dtype=torch.float32, device=logits.device)
+        stats = torch.empty((R, 4), dtype=torch.float32, device=logits.device)
+        args.loss, args.stats = loss.data_ptr(), stats.data_ptr()
+        if R:
+            _engine.launch_on(logits.device, _engine.lib().mz_distill_loss, args, 'mz_distill_loss')
+        ctx.save_for_backward(*kept, stats)
+        ctx.temperature = temperature
+        return loss
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, up):
+        *kept, stats = ctx.saved_tensors
+        args, kept = _distill_args(*kept[:4], ctx.temperature, kept[4])
+        up = up.to(torch.float32).contiguous()
+        logits = kept[0]
+        grad = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+        args.grad_loss, args.grad, args.stats = up.data_ptr(), grad.data_ptr(), stats.data_ptr()
+        if logits.shape[0]:
+            _engine.launch_on(logits.device, _engine.lib().mz_distill_grad, args, 'mz_distill_grad')
+        return grad, None, None, None, None, None
+
+
+def distillation_loss(logits: torch.Tensor, index: torch.Tensor, teacher: torch.Tensor, teacher_lse: Optional[torch.Tensor] = None,
+                      temperature: float = 1.0, weight: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Per-row distillation loss float32 [R], differentiable in logits: weight * temperature^2 * KL(p || q) with
+    q = softmax(logits / temperature) over all V actions and p the teacher's distribution over its K entries - what
+    `soft_cross_entropy` takes over whole rows, for targets that name few actions out of many.
+
+    logits [R, V], index [R, K] (int32 / int64; outside 0..V-1 = absent, the same action twice = summed), teacher [R, K] the
+    teacher's logits of those actions (-inf = probability 0).  teacher_lse float32 [R], the log-sum-exp of the teacher's
+    logits / temperature over all actions, keeps its remaining mass as one more class; without it p is renormalised over the
+    entries.  weight float32 [R]: rows of weight 0 and rows without entries have loss and gradient 0 whatever they hold.
+    A row whose logits are all -inf, or that holds NaN, gives NaN; an action of probability 0 that the teacher names gives inf."""
+    return _Distillation.apply(logits, index, teacher, teacher_lse, temperature, weight)
+
+
+def distillation_loss_grad(logits: torch.Tensor, index: torch.Tensor, teacher: torch.Tensor, teacher_lse: Optional[torch.Tensor] = None,
+                           temperature: float = 1.0, weight: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+    """`distillation_loss` and its gradient d loss[r] / d logits (type and shape of logits) in one pass that reads the logits
+    once; scale rows through `weight`.  For training loops that hand the gradient to `logits.backward(grad)` themselves."""
+    args, kept = _distill_args(logits, index, teacher, teacher_lse, temperature, weight)
+    loss = torch.empty(logits.shape[0], dtype=torch.float32, device=logits.device)
+    grad = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+    args.loss, args.grad = loss.data_ptr(), grad.data_ptr()
+    if logits.shape[0]:
+        _engine.launch_on(logits.device, _engine.lib().mz_distill_loss_grad, args, 'mz_distill_loss_grad')
+    return loss, grad
 
 
 def build_optimizer(network: nn.Module, config) -> torch.optim.Optimizer:
@@ -114,6 +201,19 @@ class Trainer:
         self.optimizer.step()
         self.training_step += 1
         return loss.item(), value_loss.item(), reward_loss.item(), policy_loss.item()
+
+    def distill(self, observations, index, teacher, teacher_lse=None, temperature: float = 1.0, weight=None) -> float:
+        """One update of the policy alone towards a teacher's top logits at the given positions (`distillation_loss`,
+        averaged over them): a cheap policy learns the moves a stronger network or the search considers."""
+        device = next(self.network.parameters()).device
+        self.update_lr()
+        policy, _, _ = self.network.initial_inference(observations.to(device), False)
+        loss = distillation_loss(policy, index, teacher, teacher_lse, temperature, weight).mean()
+        self.optimizer.zero_grad()
+        loss.backward()
+        self.optimizer.step()
+        self.training_step += 1
+        return loss.item()
 
     def step(self, batch) -> Tuple[float, float, float, float]:
         """One iteration of the training loop: schedule the learning rate, then update (trainer.py:41-45)."""
