@@ -17,7 +17,17 @@ template <typename T> __device__ __forceinline__ T narrow(acc_t<T> v) { return (
 __device__ __forceinline__ float fma_acc(float a, float b, float c) { return __builtin_fmaf(a, b, c); }
 __device__ __forceinline__ double fma_acc(double a, double b, double c) { return __builtin_fma(a, b, c); }
 
+// Workgroup barrier that orders LDS traffic only: global loads and stores in flight stay in flight across it.
+__device__ __forceinline__ void lds_fence_barrier()
+{
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+}
+
 // N elements that travel as one load or store; aligned to its size.
 template <typename T, int N> struct alignas(sizeof(T) * N) Pack { T v[N]; };
+// ... aligned to one element only (one wide access all the same: gfx950 takes any element-aligned address).
+template <typename T, int N> struct __attribute__((packed, aligned(sizeof(T)))) Loose { T v[N]; };
 
 }  // namespace mz

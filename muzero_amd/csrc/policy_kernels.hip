@@ -2,8 +2,8 @@
 // Argument checks and launches; the kernels live in the headers included below.
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
 #include <cmath>
-#include <cstring>
 
 #include "../../include/muzero_amd.h"
 #include "api.h"
@@ -17,59 +17,132 @@ static size_t size_of(int type) { return type == MZ_F64 ? 8 : type == MZ_F32 ? 4
 
 // ------------------------------------------------------------------------------------------------ recurrence
 
-template <typename T, int VEC, bool BWD> static void launch_channels(const RecurrenceArgs &q, hipStream_t st)
+// Positions a strand holds in registers; below REC_FEW_TILES channel tiles the axis is cut into segments.
+constexpr int REC_LENGTH(int size, bool backward) { return size == 8 ? 8 : backward ? 8 : 16; }
+constexpr long long REC_FEW_TILES = 128, REC_WANT_BLOCKS = 512, REC_MAX_SEGMENTS = 64;
+
+// How a recurrence is run: chosen by sizes, strides and alignment alone, for the workspace query and the call alike.
+struct RecurrencePlan {
+    bool channels, brief;    // channels contiguous; so few positions that a thread walks them all
+    int vec;                 // channels a thread holds
+    int strands, segments;
+    long long segment;
+};
+
+// VEC = 2 is a 4-byte access of a 16-bit type
+static RecurrencePlan plan_recurrence(const mz_recurrence *a, bool backward)
 {
-    constexpr int CL = 32, THREADS = 512, L = 8;
-    const long long tiles = (q.D + CL * VEC - 1) / (CL * VEC);
-    hipLaunchKernelGGL((k_recurrence_channels<T, VEC, CL, THREADS, L, BWD>), dim3((unsigned)(tiles * q.B)), dim3(THREADS), 0, st, q);
+    RecurrencePlan p{true, false, 1, REC_STRANDS, 1, a->T};
+    uint64_t low = 0;   // low bits of every address and step along the axis and the sequences
+    const int size = (int)size_of(a->type);
+    for (const mz_strided *t : {&a->gate, &a->x, &a->out, &a->y, &a->out_gate}) {
+        if (!t->p) continue;
+        if (t->stride_d != 1) p.channels = false;
+        low |= (uint64_t)(uintptr_t)t->p | (uint64_t)t->stride_b * size | (uint64_t)t->stride_t * size;
+    }
+    if (a->D == 1) p.channels = false;
+    if (!p.channels) return p;
+    auto fits = [&](int n) { return a->D % n == 0 && low % (uint64_t)(n * size) == 0; };
+    // a step, or a few: the block of strands would stand idle
+    const long long wide = 16 / size;
+    p.brief = a->T <= 8;
+    if (p.brief) {
+        p.vec = fits((int)wide) ? (int)wide : 1;
+        return p;
+    }
+    p.vec = size == 2 && fits(2) ? 2 : 1;
+    const int L = REC_LENGTH(size, backward);
+    const long long tiles = (long long)a->B * ((a->D + REC_LANES * p.vec - 1) / (REC_LANES * p.vec));
+    p.strands = (int)std::min<long long>(REC_STRANDS, std::max<long long>(2, (a->T + L - 1) / L));
+    if (tiles < REC_FEW_TILES) {
+        const long long rounds = (a->T + (long long)REC_STRANDS * L - 1) / (REC_STRANDS * L);
+        const long long want = std::min<long long>({rounds / 2, (REC_WANT_BLOCKS + tiles - 1) / tiles, REC_MAX_SEGMENTS});
+        if (want > 1) {
+            p.segment = (rounds + want - 1) / want * REC_STRANDS * L;
+            p.segments = (int)((a->T + p.segment - 1) / p.segment);
+        }
+    }
+    return p;
 }
 
-template <typename T, bool BWD> static void launch_recurrence(const RecurrenceArgs &q, bool channels, bool pairs, hipStream_t st)
+template <typename T, int VEC, bool BWD> static void launch_channels(const RecurrencePlan &p, const RecurrenceArgs &q, hipStream_t st)
 {
-    if (channels) {
-        if (sizeof(T) == 2 && pairs) launch_channels<T, 2, BWD>(q, st);
-        else launch_channels<T, 1, BWD>(q, st);
-        return;
-    }
-    constexpr int E = 4;
+    constexpr int L = REC_LENGTH((int)sizeof(T), BWD);
+    const unsigned tiles = (unsigned)((long long)q.B * ((q.D + REC_LANES * VEC - 1) / (REC_LANES * VEC)));
+    if (q.segments > 1)
+        hipLaunchKernelGGL((k_recurrence_maps<T, VEC, L, BWD>), dim3(tiles, q.segments - 1), dim3(REC_LANES * REC_STRANDS), 0, st, q);
+    hipLaunchKernelGGL((k_recurrence_channels<T, VEC, L, BWD>), dim3(tiles, q.segments), dim3(REC_LANES * p.strands), 0, st, q);
+}
+
+template <typename T, int VEC, bool BWD> static void launch_short(const RecurrenceArgs &q, hipStream_t st)
+{
+    const long long n = (long long)q.B * (q.D / VEC);
+    const unsigned threads = n >= 65536 ? 256 : 64;   // small calls: spread over the compute units
+    hipLaunchKernelGGL((k_recurrence_short<T, VEC, BWD>), dim3((unsigned)((n + threads - 1) / threads)), dim3(threads), 0, st, q);
+}
+
+template <typename T, int E, bool BWD> static void launch_rows(const RecurrenceArgs &q, hipStream_t st)
+{
     const long long need = (q.T + E - 1) / E;
     const unsigned threads = need >= 1024 ? 1024 : (unsigned)((need + 63) / 64 * 64);
     hipLaunchKernelGGL((k_recurrence_rows<T, E, BWD>), dim3((unsigned)((long long)q.B * q.D)), dim3(threads), 0, st, q);
 }
 
-template <bool BWD> static int run_recurrence(const mz_recurrence *a, void *stream, const char *fn)
+template <typename T, bool BWD> static void launch_recurrence(const RecurrencePlan &p, const RecurrenceArgs &q, hipStream_t st)
 {
-    (void)hipGetLastError();
+    constexpr int W = 16 / (int)sizeof(T);
+    if (!p.channels) {
+        if (q.T > 256) launch_rows<T, 8, BWD>(q, st);
+        else launch_rows<T, 2, BWD>(q, st);
+    } else if (p.brief) {
+        if (p.vec == W) launch_short<T, W, BWD>(q, st);
+        else launch_short<T, 1, BWD>(q, st);
+    } else if (sizeof(T) == 2 && p.vec == 2) launch_channels<T, sizeof(T) == 2 ? 2 : 1, BWD>(p, q, st);
+    else launch_channels<T, 1, BWD>(p, q, st);
+}
+
+static size_t maps_bytes(const mz_recurrence *a, const RecurrencePlan &p)
+{
+    return (size_t)(p.segments - 1) * 2 * a->B * a->D * (a->type == MZ_F64 ? 8 : 4);
+}
+
+static int check_recurrence(const mz_recurrence *a, bool backward, const char *fn)
+{
     if (!a) return api_fail(MZ_ERR_ARG, std::string(fn) + ": null argument");
     if (a->type < MZ_F32 || a->type > MZ_F64) return api_fail(MZ_ERR_ARG, std::string(fn) + ": unknown element type");
     if (a->B < 1 || a->D < 1 || a->T < 1 || (int64_t)a->B * a->D > INT32_MAX)
         return api_fail(MZ_ERR_ARG, std::string(fn) + ": sizes must be positive, and B * D below 2^31");
     if (!a->gate.p || !a->x.p || !a->out.p) return api_fail(MZ_ERR_ARG, std::string(fn) + ": null tensor");
-    if (BWD && (a->out_gate.p != nullptr) != (a->y.p != nullptr))
+    if (backward && (a->out_gate.p != nullptr) != (a->y.p != nullptr))
         return api_fail(MZ_ERR_ARG, std::string(fn) + ": the gates' gradient needs the outputs, and nothing else does");
+    return MZ_OK;
+}
+
+template <bool BWD> static int run_recurrence(const mz_recurrence *a, void *stream, const char *fn)
+{
+    (void)hipGetLastError();
+    if (int rc = check_recurrence(a, BWD, fn)) return rc;
+    const RecurrencePlan p = plan_recurrence(a, BWD);
+    if (a->workspace_bytes < (int64_t)maps_bytes(a, p) || (p.segments > 1 && !a->workspace))
+        return api_fail(MZ_ERR_ARG, std::string(fn) + ": the workspace is smaller than mz_linear_recurrence_workspace says");
     RecurrenceArgs q{};
-    q.B = a->B, q.D = a->D, q.T = a->T;
+    q.B = a->B, q.D = a->D, q.T = a->T, q.maps = a->workspace, q.segments = p.segments, q.segment = p.segment;
     // the pass runs along the axis, or against it: reversed recurrence and gradient each turn it round
     const bool turned = (a->reverse != 0) != BWD;
-    bool channels = true, pairs = q.D % 2 == 0;
     auto view = [&](const mz_strided &t) {
         RecurrenceArgs::View v{t.p, t.stride_b, t.stride_t, t.stride_d};
-        if (!t.p) return v;
-        if (q.D > 1 && t.stride_d != 1) channels = false;
-        if (((uintptr_t)t.p | (uintptr_t)(t.stride_b * 2) | (uintptr_t)(t.stride_t * 2)) % 4) pairs = false;
-        if (turned) v.p = (const char *)t.p + (q.T - 1) * t.stride_t * (int64_t)size_of(a->type), v.st = -t.stride_t;
+        if (t.p && turned) v.p = (const char *)t.p + (q.T - 1) * t.stride_t * (int64_t)size_of(a->type), v.st = -t.stride_t;
         return v;
     };
     q.a = view(a->gate), q.x = view(a->x), q.out = view(a->out);
     if (BWD) q.y = view(a->y), q.da = view(a->out_gate), q.state0 = a->y.p ? a->state : nullptr;
     q.first = BWD ? a->grad_last : a->state, q.last = BWD ? a->out_state : a->last;
-    if (q.D == 1) channels = false;
     hipStream_t st = (hipStream_t)stream;
     switch (a->type) {
-    case MZ_F32: launch_recurrence<float, BWD>(q, channels, pairs, st); break;
-    case MZ_BF16: launch_recurrence<__bf16, BWD>(q, channels, pairs, st); break;
-    case MZ_F16: launch_recurrence<_Float16, BWD>(q, channels, pairs, st); break;
-    default: launch_recurrence<double, BWD>(q, channels, pairs, st);
+    case MZ_F32: launch_recurrence<float, BWD>(p, q, st); break;
+    case MZ_BF16: launch_recurrence<__bf16, BWD>(p, q, st); break;
+    case MZ_F16: launch_recurrence<_Float16, BWD>(p, q, st); break;
+    default: launch_recurrence<double, BWD>(p, q, st);
     }
     return api_launch_status(fn);
 }
@@ -82,6 +155,14 @@ extern "C" int mz_linear_recurrence(const mz_recurrence *args_h, void *stream)
 extern "C" int mz_linear_recurrence_backward(const mz_recurrence *args_h, void *stream)
 {
     return run_recurrence<true>(args_h, stream, "mz_linear_recurrence_backward");
+}
+
+extern "C" int mz_linear_recurrence_workspace(const mz_recurrence *args_h, int32_t backward, int64_t *out_bytes)
+{
+    if (int rc = check_recurrence(args_h, backward != 0, "mz_linear_recurrence_workspace")) return rc;
+    if (!out_bytes) return api_fail(MZ_ERR_ARG, "mz_linear_recurrence_workspace: null argument");
+    *out_bytes = (int64_t)maps_bytes(args_h, plan_recurrence(args_h, backward != 0));
+    return MZ_OK;
 }
 
 // ------------------------------------------------------------------------------------------------ distillation

@@ -25,6 +25,9 @@ struct RecurrenceArgs {
     const void *first;   // acc[B][D] what goes into position 0 (backward: gradient of the last state), NULL = 0
     const void *state0;  // backward: acc[B][D] the forward pass's first state, NULL = 0
     void *last;          // acc[B][D] the state behind the last position (backward: gradient of the first state), may be NULL
+    void *maps;          // acc[segments - 1][2][B][D] maps of all segments but the last, or NULL: one segment
+    int segments;
+    long long segment;   // positions per segment
 };
 
 template <typename T> __device__ __forceinline__ const T *at(const RecurrenceArgs::View &v, int b, long long s, int d)
@@ -32,89 +35,270 @@ template <typename T> __device__ __forceinline__ const T *at(const RecurrenceArg
     return (const T *)v.p + (long long)b * v.sb + s * v.st + (long long)d * v.sd;
 }
 
-// Channels contiguous: CL neighbouring lanes hold CL * VEC neighbouring channels, and each such group of lanes ("strand")
-// walks L consecutive positions in registers; the block's NV strands follow each other in time and exchange their maps
-// through LDS, one barrier per NV * L positions.
-template <typename T, int VEC, int CL, int THREADS, int L, bool BWD>
-__global__ __launch_bounds__(THREADS) void k_recurrence_channels(RecurrenceArgs q)
-{
-    using A = acc_t<T>;
+template <typename A> __device__ __forceinline__ A state_at(const void *p, long long i) { return p ? ((const A *)p)[i] : A(0); }
+
+// L positions of one strand in registers, all loads asked for at once.
+template <typename T, int VEC, int L, bool BWD> struct Strand {
     using P = Pack<T, VEC>;
-    constexpr int NV = THREADS / CL;
-    __shared__ A run_a[2][NV][CL * VEC], run_x[2][NV][CL * VEC];
-    const int tiles = (q.D + CL * VEC - 1) / (CL * VEC);
-    const int b = blockIdx.x / tiles, c = (threadIdx.x % CL) * VEC, d = (blockIdx.x % tiles) * CL * VEC + c;
-    const int v = threadIdx.x / CL;
-    const bool live = d < q.D;
-    A carry[VEC];
-#pragma unroll
-    for (int j = 0; j < VEC; j++) carry[j] = live && q.first ? ((const A *)q.first)[(long long)b * q.D + d + j] : A(0);
-    const bool want_da = BWD && q.da.p;
-    int buf = 0;
-    for (long long base = 0; base < q.T; base += NV * L, buf ^= 1) {
-        const long long s0 = base + v * L;
-        P a[L], x[L], y[L];
+    P a[L], x[L], y[BWD ? L : 1];
+
+    // FULL: every position is below the end (and, backward, so is the one behind it); otherwise addresses are clamped and
+    // positions from `end` on become the identity map.
+    template <bool FULL>
+    __device__ __forceinline__ void load(const RecurrenceArgs &q, int b, long long s0, long long end, int d, bool want_da)
+    {
 #pragma unroll
         for (int i = 0; i < L; i++) {
-            const long long s = s0 + i;
-            if (live && s < q.T) {
-                x[i] = *(const P *)at<T>(q.x, b, s, d);
-                if (!BWD || s > 0) a[i] = *(const P *)at<T>(q.a, b, BWD ? s - 1 : s, d);
-                else
-#pragma unroll
-                    for (int j = 0; j < VEC; j++) a[i].v[j] = T(1.0f);
-                if (want_da && s + 1 < q.T) y[i] = *(const P *)at<T>(q.y, b, s + 1, d);
-            } else
-#pragma unroll
-                for (int j = 0; j < VEC; j++) a[i].v[j] = T(1.0f), x[i].v[j] = T(0.0f);
+            const long long s = FULL ? s0 + i : min(s0 + i, q.T - 1);
+            x[i] = *(const P *)at<T>(q.x, b, s, d);
+            a[i] = *(const P *)at<T>(q.a, b, !BWD ? s : FULL && i ? s - 1 : max(s - 1, 0ll), d);
         }
-        A ra[VEC], rx[VEC];
+        if constexpr (BWD) {
+            if (want_da)
 #pragma unroll
-        for (int j = 0; j < VEC; j++) {
-            ra[j] = A(1), rx[j] = A(0);
+                for (int i = 0; i < L; i++) y[i] = *(const P *)at<T>(q.y, b, FULL ? s0 + i + 1 : min(s0 + i + 1, q.T - 1), d);
+            if (s0 == 0)
 #pragma unroll
-            for (int i = 0; i < L; i++) {
+                for (int j = 0; j < VEC; j++) a[0].v[j] = T(1.0f);   // nothing precedes the first position: its carry enters as it is
+        }
+        if (!FULL)
+#pragma unroll
+            for (int i = 0; i < L; i++)
+                if (s0 + i >= end)
+#pragma unroll
+                    for (int j = 0; j < VEC; j++) a[i].v[j] = T(1.0f), x[i].v[j] = T(0.0f);
+    }
+    // The strand's map behind the map (ra, rx).
+    __device__ __forceinline__ void compose(acc_t<T> (&ra)[VEC], acc_t<T> (&rx)[VEC]) const
+    {
+#pragma unroll
+        for (int i = 0; i < L; i++)
+#pragma unroll
+            for (int j = 0; j < VEC; j++) {
                 rx[j] = fma_acc(widen(a[i].v[j]), rx[j], widen(x[i].v[j]));
                 ra[j] *= widen(a[i].v[j]);
             }
-            run_a[buf][v][c + j] = ra[j], run_x[buf][v][c + j] = rx[j];
-        }
-        __syncthreads();
-        A h[VEC];
+    }
+};
+
+constexpr int REC_LANES = 32, REC_STRANDS = 16;   // lanes along the channels, strands of a block
+
+// Channels contiguous: 32 neighbouring lanes hold 32 * VEC neighbouring channels (128 bytes of a position) and walk L
+// consecutive positions in registers; the block's strands follow each other in time and exchange their maps through LDS,
+// one barrier per round of strands, while the next round's loads are on their way.
+// A grid of few channel tiles leaves compute units idle: the axis is then cut into segments of one block each, whose maps
+// k_recurrence_maps has left in memory; a block folds those of the segments before its own.
+template <typename T, int VEC, int L, bool BWD>
+__global__ __launch_bounds__(REC_LANES * REC_STRANDS) void k_recurrence_channels(RecurrenceArgs q)
+{
+    using A = acc_t<T>;
+    using P = Pack<T, VEC>;
+    struct Map { A a[VEC], x[VEC]; };
+    __shared__ Map run[2][REC_STRANDS][REC_LANES];
+    const int nv = blockDim.x / REC_LANES;
+    const int tiles = (q.D + REC_LANES * VEC - 1) / (REC_LANES * VEC);
+    // segments of one tile run from the last to the first: what the maps' pass read last is read first
+    const int seg = q.segments - 1 - blockIdx.y;
+    const int b = blockIdx.x / tiles, c = threadIdx.x % REC_LANES, v = threadIdx.x / REC_LANES;
+    const int d0 = (blockIdx.x % tiles) * REC_LANES * VEC + c * VEC;
+    const bool live = d0 < q.D;
+    const int d = live ? d0 : q.D - VEC;   // idle lanes read what the last live one reads
+    const long long row = (long long)b * q.D + d;
+    const long long begin = seg * q.segment, end = min(begin + q.segment, q.T);
+    const bool want_da = BWD && q.da.p;
+    A carry[VEC];
 #pragma unroll
-        for (int j = 0; j < VEC; j++)
-#pragma unroll 8
-            for (int i = 0; i < NV; i++) {
-                if (i == v) h[j] = carry[j];
-                carry[j] = fma_acc(run_a[buf][i][c + j], carry[j], run_x[buf][i][c + j]);
+    for (int j = 0; j < VEC; j++) carry[j] = state_at<A>(q.first, row + j);
+    const long long rows = (long long)q.B * q.D;
+#pragma unroll 4
+    for (int i = 0; i < seg; i++) {
+        const A *m = (const A *)q.maps + (long long)i * 2 * rows + row;
+#pragma unroll
+        for (int j = 0; j < VEC; j++) carry[j] = fma_acc(m[j], carry[j], m[rows + j]);
+    }
+    const int round = nv * L;
+    int buf = 0;
+    Strand<T, VEC, L, BWD> now, next;
+    const long long inside = BWD ? min(end, q.T - 1) : end;   // a round that ends here or earlier needs no clamping
+    auto load = [&](Strand<T, VEC, L, BWD> &w, long long base) {
+        if (base + round <= inside) w.template load<true>(q, b, base + v * L, end, d, want_da);
+        else w.template load<false>(q, b, base + v * L, end, d, want_da);
+    };
+    load(now, begin);
+    for (long long base = begin; base < end; base += round, buf ^= 1) {
+        const bool more = base + round < end;
+        if (more) load(next, base + round);
+        Map m;
+#pragma unroll
+        for (int j = 0; j < VEC; j++) m.a[j] = A(1), m.x[j] = A(0);
+        now.compose(m.a, m.x);
+        run[buf][v][c] = m;
+        lds_fence_barrier();
+        A h[VEC];
+        for (int i = 0; i < nv; i++) {
+            const Map o = run[buf][i][c];
+#pragma unroll
+            for (int j = 0; j < VEC; j++) {
+                h[j] = i == v ? carry[j] : h[j];
+                carry[j] = fma_acc(o.a[j], carry[j], o.x[j]);
             }
+        }
+        const long long s0 = base + v * L;
+        const int left = live ? (int)min((long long)L, max(end - s0, 0ll)) : 0;
 #pragma unroll
         for (int i = 0; i < L; i++) {
-            const long long s = s0 + i;
-            if (!live || s >= q.T) continue;
+            if (i >= left) break;
             P o, da;
 #pragma unroll
             for (int j = 0; j < VEC; j++) {
-                h[j] = fma_acc(widen(a[i].v[j]), h[j], widen(x[i].v[j]));
+                h[j] = fma_acc(widen(now.a[i].v[j]), h[j], widen(now.x[i].v[j]));
                 o.v[j] = narrow<T>(h[j]);
+            }
+            *(P *)at<T>(q.out, b, s0 + i, d) = o;
+            if constexpr (BWD) {
                 if (want_da) {
-                    const A before = s + 1 < q.T ? widen(y[i].v[j]) : q.state0 ? ((const A *)q.state0)[(long long)b * q.D + d + j] : A(0);
-                    da.v[j] = narrow<T>(h[j] * before);
+                    const bool first = s0 + i + 1 == q.T;   // of the forward pass: what precedes it is the first state
+#pragma unroll
+                    for (int j = 0; j < VEC; j++) {
+                        const A before = first ? state_at<A>(q.state0, row + j) : widen(now.y[i].v[j]);
+                        da.v[j] = narrow<T>(h[j] * before);
+                    }
+                    *(P *)at<T>(q.da, b, s0 + i, d) = da;
                 }
             }
-            *(P *)at<T>(q.out, b, s, d) = o;
-            if (want_da) *(P *)at<T>(q.da, b, s, d) = da;
         }
+        if (more) now = next;
     }
-    if (q.last && live && v == 0) {
+    if (q.last && live && v == 0 && seg == q.segments - 1) {
 #pragma unroll
         for (int j = 0; j < VEC; j++) {
             A z = carry[j];
             if (BWD) z *= widen(at<T>(q.a, b, q.T - 1, d)[j]);
-            ((A *)q.last)[(long long)b * q.D + d + j] = z;
+            ((A *)q.last)[row + j] = z;
         }
     }
 }
+
+// The maps of all segments but the last: every strand of a block composes a stretch of its own, and the first strand folds
+// the stretches.
+template <typename T, int VEC, int L, bool BWD>
+__global__ __launch_bounds__(REC_LANES * REC_STRANDS) void k_recurrence_maps(RecurrenceArgs q)
+{
+    using A = acc_t<T>;
+    struct Map { A a[VEC], x[VEC]; };
+    __shared__ Map run[REC_STRANDS][REC_LANES];
+    const int tiles = (q.D + REC_LANES * VEC - 1) / (REC_LANES * VEC);
+    const int seg = blockIdx.y;
+    const int b = blockIdx.x / tiles, c = threadIdx.x % REC_LANES, v = threadIdx.x / REC_LANES;
+    const int d0 = (blockIdx.x % tiles) * REC_LANES * VEC + c * VEC;
+    const bool live = d0 < q.D;
+    const int d = live ? d0 : q.D - VEC;
+    const long long stretch = ((q.segment + REC_STRANDS - 1) / REC_STRANDS + L - 1) / L * L;
+    const long long last = (seg + 1) * q.segment;   // below T: the last segment's map is not needed
+    const long long begin = min(seg * q.segment + v * stretch, last), end = min(begin + stretch, last);
+    Map m;
+#pragma unroll
+    for (int j = 0; j < VEC; j++) m.a[j] = A(1), m.x[j] = A(0);
+    Strand<T, VEC, L, BWD> now, next;
+    auto load = [&](Strand<T, VEC, L, BWD> &w, long long s) {
+        if (s + L <= end) w.template load<true>(q, b, s, end, d, false);
+        else w.template load<false>(q, b, s, end, d, false);
+    };
+    if (begin < end) load(now, begin);
+    for (long long s = begin; s < end; s += L) {
+        const bool more = s + L < end;
+        if (more) load(next, s + L);
+        now.compose(m.a, m.x);
+        if (more) now = next;
+    }
+    run[v][c] = m;
+    __syncthreads();
+    if (v == 0 && live) {
+        for (int i = 1; i < REC_STRANDS; i++) {
+            const Map o = run[i][c];
+#pragma unroll
+            for (int j = 0; j < VEC; j++) m.x[j] = fma_acc(o.a[j], m.x[j], o.x[j]), m.a[j] *= o.a[j];
+        }
+        const long long rows = (long long)q.B * q.D;
+        A *to = (A *)q.maps + (long long)seg * 2 * rows + (long long)b * q.D + d;
+#pragma unroll
+        for (int j = 0; j < VEC; j++) to[j] = m.a[j], to[rows + j] = m.x[j];
+    }
+}
+
+// Few positions (a step of serving, short records): a thread walks VEC channels of one sequence through all of them.
+template <typename T, int VEC, bool BWD>
+__global__ __launch_bounds__(256) void k_recurrence_short(RecurrenceArgs q)
+{
+    using A = acc_t<T>;
+    using P = Pack<T, VEC>;
+    constexpr int L = 4;
+    const int per = q.D / VEC;
+    const long long id = (long long)blockIdx.x * blockDim.x + threadIdx.x;
+    if (id >= (long long)per * q.B) return;
+    const int b = (int)(id / per), d = (int)(id % per) * VEC;
+    const long long row = (long long)b * q.D + d;
+    const bool want_da = BWD && q.da.p;
+    A h[VEC];
+#pragma unroll
+    for (int j = 0; j < VEC; j++) h[j] = state_at<A>(q.first, row + j);
+    for (long long s0 = 0; s0 < q.T; s0 += L) {
+        Strand<T, VEC, L, BWD> w;
+        w.template load<false>(q, b, s0, q.T, d, want_da);
+#pragma unroll
+        for (int i = 0; i < L; i++) {
+            if (s0 + i >= q.T) break;
+            P o, da;
+#pragma unroll
+            for (int j = 0; j < VEC; j++) {
+                h[j] = fma_acc(widen(w.a[i].v[j]), h[j], widen(w.x[i].v[j]));
+                o.v[j] = narrow<T>(h[j]);
+            }
+            *(P *)at<T>(q.out, b, s0 + i, d) = o;
+            if constexpr (BWD) {
+                if (want_da) {
+                    const bool first = s0 + i + 1 == q.T;
+#pragma unroll
+                    for (int j = 0; j < VEC; j++) {
+                        const A before = first ? state_at<A>(q.state0, row + j) : widen(w.y[i].v[j]);
+                        da.v[j] = narrow<T>(h[j] * before);
+                    }
+                    *(P *)at<T>(q.da, b, s0 + i, d) = da;
+                }
+            }
+        }
+    }
+    if (q.last)
+#pragma unroll
+        for (int j = 0; j < VEC; j++)
+            ((A *)q.last)[row + j] = BWD ? h[j] * widen(at<T>(q.a, b, q.T - 1, d)[j]) : h[j];
+}
+
+// E consecutive positions of one row; one wide access where they are neighbours in memory (st = 1 or -1).
+template <typename T, int E> struct Stretch {
+    T v[E];
+    __device__ __forceinline__ void load(const RecurrenceArgs::View &w, const T *row, long long s, long long T_, T fill)
+    {
+        if (s >= 0 && s + E <= T_ && (w.st == 1 || w.st == -1)) {
+            const Loose<T, E> p = *(const Loose<T, E> *)(row + (w.st == 1 ? s : -(s + E - 1)));
+#pragma unroll
+            for (int i = 0; i < E; i++) v[i] = w.st == 1 ? p.v[i] : p.v[E - 1 - i];
+        } else
+#pragma unroll
+            for (int i = 0; i < E; i++) v[i] = s + i >= 0 && s + i < T_ ? row[(s + i) * w.st] : fill;
+    }
+    __device__ __forceinline__ void store(const RecurrenceArgs::View &w, T *row, long long s, long long T_) const
+    {
+        if (s + E <= T_ && (w.st == 1 || w.st == -1)) {
+            Loose<T, E> p;
+#pragma unroll
+            for (int i = 0; i < E; i++) p.v[i] = w.st == 1 ? v[i] : v[E - 1 - i];
+            *(Loose<T, E> *)(row + (w.st == 1 ? s : -(s + E - 1))) = p;
+        } else
+#pragma unroll
+            for (int i = 0; i < E; i++) if (s + i < T_) row[(s + i) * w.st] = v[i];
+    }
+};
 
 // Any strides, one row (b, d) per block: every thread walks E consecutive positions, the maps are composed across the wave
 // by shuffles and across the waves through LDS.
@@ -124,26 +308,25 @@ __global__ __launch_bounds__(1024) void k_recurrence_rows(RecurrenceArgs q)
     using A = acc_t<T>;
     __shared__ A run_a[2][16], run_x[2][16];
     const int b = blockIdx.x / q.D, d = blockIdx.x % q.D, lane = threadIdx.x % 64, w = threadIdx.x / 64, nw = blockDim.x / 64;
-    A carry = q.first ? ((const A *)q.first)[blockIdx.x] : A(0);
-    const A state0 = BWD && q.state0 ? ((const A *)q.state0)[blockIdx.x] : A(0);
+    A carry = state_at<A>(q.first, blockIdx.x);
     const bool want_da = BWD && q.da.p;
     int buf = 0;
     for (long long base = 0; base < q.T; base += (long long)blockDim.x * E, buf ^= 1) {
         const long long s0 = base + (long long)threadIdx.x * E;
-        A a[E], x[E], y[E];
+        Stretch<T, E> a, x, y;
+        x.load(q.x, at<T>(q.x, b, 0, d), s0, q.T, T(0.0f));
+        // a position behind the end is the identity map; backward, the one in front of the first as well
+        if (!BWD) a.load(q.a, at<T>(q.a, b, 0, d), s0, q.T, T(1.0f));
+        else {
+            a.load(q.a, at<T>(q.a, b, 0, d), s0 - 1, q.T, T(1.0f));
+            if (want_da) y.load(q.y, at<T>(q.y, b, 0, d), s0 + 1, q.T, T(0.0f));
+            if (s0 + E > q.T)
+#pragma unroll
+                for (int i = 0; i < E; i++) if (s0 + i >= q.T) a.v[i] = T(1.0f);
+        }
         A ra = A(1), rx = A(0);
 #pragma unroll
-        for (int i = 0; i < E; i++) {
-            const long long s = s0 + i;
-            a[i] = A(1), x[i] = A(0), y[i] = state0;
-            if (s < q.T) {
-                x[i] = widen(*at<T>(q.x, b, s, d));
-                if (!BWD || s > 0) a[i] = widen(*at<T>(q.a, b, BWD ? s - 1 : s, d));
-                if (want_da && s + 1 < q.T) y[i] = widen(*at<T>(q.y, b, s + 1, d));
-            }
-        }
-#pragma unroll
-        for (int i = 0; i < E; i++) rx = fma_acc(a[i], rx, x[i]), ra *= a[i];
+        for (int i = 0; i < E; i++) rx = fma_acc(widen(a.v[i]), rx, widen(x.v[i])), ra *= widen(a.v[i]);
 #pragma unroll
         for (int k = 1; k < 64; k *= 2) {
             const A pa = __shfl_up(ra, k), px = __shfl_up(rx, k);
@@ -152,20 +335,26 @@ __global__ __launch_bounds__(1024) void k_recurrence_rows(RecurrenceArgs q)
         if (lane == 63) run_a[buf][w] = ra, run_x[buf][w] = rx;
         A ea = __shfl_up(ra, 1), ex = __shfl_up(rx, 1);
         if (lane == 0) ea = A(1), ex = A(0);
-        __syncthreads();
+        lds_fence_barrier();
         A h = carry;
         for (int i = 0; i < nw; i++) {
             if (i == w) h = carry;
             carry = fma_acc(run_a[buf][i], carry, run_x[buf][i]);
         }
         h = fma_acc(ea, h, ex);
+        if (s0 >= q.T) continue;
+        Stretch<T, E> o, da;
 #pragma unroll
         for (int i = 0; i < E; i++) {
-            const long long s = s0 + i;
-            if (s >= q.T) break;
-            h = fma_acc(a[i], h, x[i]);
-            *(T *)at<T>(q.out, b, s, d) = narrow<T>(h);
-            if (want_da) *(T *)at<T>(q.da, b, s, d) = narrow<T>(h * y[i]);
+            h = fma_acc(widen(a.v[i]), h, widen(x.v[i]));
+            o.v[i] = narrow<T>(h);
+            if constexpr (BWD) {
+                if (want_da) da.v[i] = narrow<T>(h * (s0 + i + 1 == q.T ? state_at<A>(q.state0, blockIdx.x) : widen(y.v[i])));
+            }
+        }
+        o.store(q.out, (T *)at<T>(q.out, b, 0, d), s0, q.T);
+        if constexpr (BWD) {
+            if (want_da) da.store(q.da, (T *)at<T>(q.da, b, 0, d), s0, q.T);
         }
     }
     if (q.last && threadIdx.x == 0) {

@@ -58,10 +58,10 @@ def verify_drafts(tokens: torch.Tensor, draft: Optional[torch.Tensor], target: t
         draft = draft.contiguous()
     tokens, u_accept, u_sample = tokens.contiguous(), u_accept.contiguous(), u_sample.contiguous()
     lengths = None if lengths is None else lengths.contiguous()
-    p = lambda t: None if t is None else t.data_ptr()  # noqa: E731
+    p = lambda t: 0 if t is None else t.data_ptr()  # noqa: E731
     sd = (0, 0) if draft is None else draft.stride()[:2]
-    args = _engine.MzVerify(_engine.ELEMENT_TYPES[target.dtype], int(tokens.dtype == torch.int64), B, K, V, 0, p(tokens), p(draft),
-                            *sd, p(target), target.stride(0), target.stride(1), p(u_accept), p(u_sample), p(lengths),
-                            p(accepted), p(out))
+    args = _engine.PACK_VERIFY(_engine.ELEMENT_TYPES[target.dtype], int(tokens.dtype == torch.int64), B, K, V, 0, p(tokens), p(draft),
+                               *sd, p(target), target.stride(0), target.stride(1), p(u_accept), p(u_sample), p(lengths),
+                               p(accepted), p(out))
     _engine.launch_on(target.device, _engine.lib().mz_verify_drafts, args, 'mz_verify_drafts')
     return accepted, out

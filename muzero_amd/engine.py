@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import ctypes as C
 import os
+import struct
 
 import numpy as np
 import torch
@@ -60,7 +61,8 @@ class MzStrided(C.Structure):
 class MzRecurrence(C.Structure):
     _fields_ = [('type', C.c_int32), ('B', C.c_int32), ('D', C.c_int32), ('reverse', C.c_int32), ('T', C.c_int64),
                 ('gate', MzStrided), ('x', MzStrided), ('out', MzStrided), ('y', MzStrided), ('out_gate', MzStrided),
-                ('state', C.c_void_p), ('last', C.c_void_p), ('grad_last', C.c_void_p), ('out_state', C.c_void_p)]
+                ('state', C.c_void_p), ('last', C.c_void_p), ('grad_last', C.c_void_p), ('out_state', C.c_void_p),
+                ('workspace', C.c_void_p), ('workspace_bytes', C.c_int64)]
 
 
 class MzDistill(C.Structure):
@@ -79,13 +81,18 @@ class MzVerify(C.Structure):
 
 
 ENV_TICTACTOE, ENV_CARTPOLE = 1, 2
+# The same layouts as flat packers: the tensor operators' calls are short enough for the fields of a ctypes structure, set one
+# by one, to cost more than the launch.
+PACK_RECURRENCE = struct.Struct('@4iq20q6q').pack
+PACK_DISTILL = struct.Struct('@6if10q').pack
+PACK_VERIFY = struct.Struct('@6i12q').pack
 # element types of the tensor operators (MZ_F32 ...)
 ELEMENT_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2, torch.float64: 3}
 
 EXPORTS = ['mz_create', 'mz_destroy', 'mz_last_error', 'mz_set_seed', 'mz_check', 'mz_root_prepare', 'mz_tree_reset', 'mz_select',
            'mz_select_outputs', 'mz_expand_backup', 'mz_to_act', 'mz_search_run', 'mz_search_run_act', 'mz_search_move', 'mz_set_network', 'mz_set_root_network', 'mz_search_begin_net', 'mz_set_network_mfma', 'mz_set_root_network_mfma', 'mz_initial_inference_mfma', 'mz_expand_backup_net', 'mz_expand_backup_net_static', 'mz_act_env_step', 'mz_act_env_step_log', 'mz_log_count_games', 'mz_log_list_games', 'mz_tree_export',
            'mz_stats', 'mz_node_qtransform', 'mz_node_select', 'mz_node_backward', 'mz_tree_import', 'mz_considered_visits', 'mz_legacy_root_noise', 'mz_legacy_gumbel', 'mz_make_targets', 'mz_scalar_to_support',
-           'mz_linear_recurrence', 'mz_linear_recurrence_backward', 'mz_distill_loss', 'mz_distill_grad',
+           'mz_linear_recurrence', 'mz_linear_recurrence_backward', 'mz_linear_recurrence_workspace', 'mz_distill_loss', 'mz_distill_grad',
            'mz_distill_loss_grad', 'mz_verify_drafts', 'mz_version']
 
 
@@ -136,10 +143,10 @@ def lib():
         L.mz_node_qtransform.argtypes = [vp, i32, i32, i32, vp, vp]
         L.mz_node_select.argtypes = [vp, i32, i32, i32, vp, vp, vp]
         L.mz_considered_visits.argtypes = [i32, i32, vp]
-        for name, struct in (('mz_linear_recurrence', MzRecurrence), ('mz_linear_recurrence_backward', MzRecurrence),
-                             ('mz_distill_loss', MzDistill), ('mz_distill_grad', MzDistill),
-                             ('mz_distill_loss_grad', MzDistill), ('mz_verify_drafts', MzVerify)):
-            getattr(L, name).argtypes = [C.POINTER(struct), vp]
+        for name in ('mz_linear_recurrence', 'mz_linear_recurrence_backward', 'mz_distill_loss', 'mz_distill_grad',
+                     'mz_distill_loss_grad', 'mz_verify_drafts'):
+            getattr(L, name).argtypes = [vp, vp]
+        L.mz_linear_recurrence_workspace.argtypes = [vp, i32, vp]
         _lib = L
     return _lib
 
@@ -228,13 +235,14 @@ def _stream():
     return C.c_void_p(torch.cuda.current_stream().cuda_stream)
 
 
-def launch_on(device, fn, struct, what):
-    """Calls a tensor operator's entry point on the current stream of `device`, which need not be the current one."""
+def launch_on(device, fn, args: bytes, what):
+    """Calls a tensor operator's entry point with a packed argument struct, on the current stream of `device`, which need not
+    be the current one."""
     if device.index == torch.cuda.current_device():
-        _check(fn(C.byref(struct), _stream()), what)
+        _check(fn(args, _stream()), what)
     else:
         with torch.cuda.device(device):
-            _check(fn(C.byref(struct), _stream()), what)
+            _check(fn(args, _stream()), what)
 
 
 class SearchEngine:

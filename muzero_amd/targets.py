@@ -104,10 +104,6 @@ def scalar_to_support(x: torch.Tensor, support_limit: int) -> torch.Tensor:
 _STATE_TYPE = {torch.float64: torch.float64}
 
 
-def _strided(t) -> '_engine.MzStrided':
-    return _engine.MzStrided(t.data_ptr(), *t.stride())
-
-
 def _lined_up(t: torch.Tensor, channels: bool) -> torch.Tensor:
     """`t` itself where the kernels read its layout well: channels contiguous, or (one channel, or time contiguous) any."""
     return t.contiguous() if channels and t.stride(2) != 1 else t
@@ -128,11 +124,23 @@ def _recurrence_call(backward, gate, x, state, reverse, out, last=None, y=None, 
             views = [gate, x, out, y, out_gate]
         else:
             B, D = 1, B
-    none = _engine.MzStrided()
-    p = lambda t: None if t is None else t.data_ptr()  # noqa: E731
-    args = _engine.MzRecurrence(_engine.ELEMENT_TYPES[x.dtype], B, D, int(reverse), T,
-                                *[none if v is None else _strided(v) for v in views], p(state), p(last), p(grad_last), p(out_state))
+    fields = []
+    for v in views:
+        if v is None:
+            fields += (0, 0, 0, 0)
+        else:
+            fields += (v.data_ptr(), *v.stride())
+    for v in (state, last, grad_last, out_state):
+        fields.append(0 if v is None else v.data_ptr())
+    head = (_engine.ELEMENT_TYPES[x.dtype], B, D, int(reverse), T)
     L = lib()
+    need = 0
+    if T > 256:   # shorter records are never cut into segments
+        size = C.c_int64()
+        _check(L.mz_linear_recurrence_workspace(_engine.PACK_RECURRENCE(*head, *fields, 0, 0), int(backward), C.byref(size)))
+        need = size.value
+    space = torch.empty(need, dtype=torch.uint8, device=x.device) if need else None
+    args = _engine.PACK_RECURRENCE(*head, *fields, space.data_ptr() if need else 0, need)
     if backward:
         _engine.launch_on(x.device, L.mz_linear_recurrence_backward, args, 'mz_linear_recurrence_backward')
     else:

@@ -50,7 +50,7 @@ def soft_cross_entropy(logits: torch.Tensor, target: torch.Tensor) -> torch.Tens
 
 
 def _distill_args(logits, index, teacher, teacher_lse, temperature, weight):
-    """Checks the arguments of the distillation calls; returns (MzDistill without outputs, tensors it points to)."""
+    """Checks the arguments of the distillation calls."""
     for name, t in (('logits', logits), ('index', index), ('teacher', teacher), ('teacher_lse', teacher_lse), ('weight', weight)):
         if t is None and name in ('teacher_lse', 'weight'):
             continue
@@ -74,37 +74,43 @@ def _distill_args(logits, index, teacher, teacher_lse, temperature, weight):
     logits, index, teacher = logits.detach(), index.contiguous(), teacher.detach().contiguous()
     lse = None if teacher_lse is None else teacher_lse.detach().contiguous()
     weight = None if weight is None else weight.detach().contiguous()
-    p = lambda t: None if t is None else t.data_ptr()  # noqa: E731
-    args = _engine.MzDistill(types[logits.dtype], types[teacher.dtype], int(index.dtype == torch.int64), R, V, K,
-                             float(temperature), p(logits), logits.stride(0), p(index), p(teacher), p(lse), p(weight))
-    return args, (logits, index, teacher, lse, weight)
+    return _Call(logits, index, teacher, lse, weight, float(temperature))
+
+
+class _Call:
+    """Checked arguments of a distillation call and the tensors they point to."""
+
+    def __init__(self, logits, index, teacher, lse, weight, temperature):
+        self.kept, self.temperature = (logits, index, teacher, lse, weight), temperature
+
+    def run(self, what, grad_loss=None, loss=None, grad=None, stats=None):
+        logits, index, teacher, lse, weight = self.kept
+        types = _engine.ELEMENT_TYPES
+        args = _engine.PACK_DISTILL(types[logits.dtype], types[teacher.dtype], int(index.dtype == torch.int64), *logits.shape,
+                                    index.shape[1], self.temperature, logits.data_ptr(), logits.stride(0),
+                                    *[0 if t is None else t.data_ptr() for t in (index, teacher, lse, weight, grad_loss, loss, grad, stats)])
+        if logits.shape[0]:
+            _engine.launch_on(logits.device, getattr(_engine.lib(), what), args, what)
 
 
 class _Distillation(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, index, teacher, teacher_lse, temperature, weight):
-        args, kept = _distill_args(logits, index, teacher, teacher_lse, temperature, weight)
-        R = logits.shape[0]
-        loss = torch.empty(R, dtype=torch.float32, device=logits.device)
-        stats = torch.empty((R, 4), dtype=torch.float32, device=logits.device)
-        args.loss, args.stats = loss.data_ptr(), stats.data_ptr()
-        if R:
-            _engine.launch_on(logits.device, _engine.lib().mz_distill_loss, args, 'mz_distill_loss')
-        ctx.save_for_backward(*kept, stats)
-        ctx.temperature = temperature
+        call = _distill_args(logits, index, teacher, teacher_lse, temperature, weight)
+        loss = torch.empty(logits.shape[0], dtype=torch.float32, device=logits.device)
+        stats = torch.empty((logits.shape[0], 4), dtype=torch.float32, device=logits.device)
+        call.run('mz_distill_loss', loss=loss, stats=stats)
+        ctx.save_for_backward(*call.kept, stats)
+        ctx.temperature = call.temperature
         return loss
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, up):
         *kept, stats = ctx.saved_tensors
-        args, kept = _distill_args(*kept[:4], ctx.temperature, kept[4])
-        up = up.to(torch.float32).contiguous()
         logits = kept[0]
         grad = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
-        args.grad_loss, args.grad, args.stats = up.data_ptr(), grad.data_ptr(), stats.data_ptr()
-        if logits.shape[0]:
-            _engine.launch_on(logits.device, _engine.lib().mz_distill_grad, args, 'mz_distill_grad')
+        _Call(*kept, ctx.temperature).run('mz_distill_grad', grad_loss=up.to(torch.float32).contiguous(), grad=grad, stats=stats)
         return grad, None, None, None, None, None
 
 
@@ -126,12 +132,10 @@ def distillation_loss_grad(logits: torch.Tensor, index: torch.Tensor, teacher: t
                            temperature: float = 1.0, weight: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
     """`distillation_loss` and its gradient d loss[r] / d logits (type and shape of logits) in one pass that reads the logits
     once; scale rows through `weight`.  For training loops that hand the gradient to `logits.backward(grad)` themselves."""
-    args, kept = _distill_args(logits, index, teacher, teacher_lse, temperature, weight)
+    call = _distill_args(logits, index, teacher, teacher_lse, temperature, weight)
     loss = torch.empty(logits.shape[0], dtype=torch.float32, device=logits.device)
     grad = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
-    args.loss, args.grad = loss.data_ptr(), grad.data_ptr()
-    if logits.shape[0]:
-        _engine.launch_on(logits.device, _engine.lib().mz_distill_loss_grad, args, 'mz_distill_loss_grad')
+    call.run('mz_distill_loss_grad', loss=loss, grad=grad)
     return loss, grad
 
 
