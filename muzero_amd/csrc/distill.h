@@ -43,256 +43,461 @@ __device__ __forceinline__ int entry_at(const DistillArgs &q, long long i)
 }
 
 
-// The teacher's side of a row, in LDS: what one wave makes of the K entries.
-struct Entries {
-    int *index;      // [K] action of the entry, -1: absent
-    double *p;       // [K] the entry's probability
-    double *total;   // [K] probability of its action over all entries that name it; < 0: not the first of them
-    double mass, ent, rest;   // sum p, sum p log p, 1 - mass (>= 0; 0 without lse)
-    bool some;
-};
 
-__device__ __forceinline__ double wave_sum(double v)
+template <int G> __device__ __forceinline__ double group_sum(double v)
 {
-    for (int k = 32; k; k /= 2) v += __shfl_xor(v, k);
+#pragma unroll
+    for (int k = G / 2; k; k /= 2) v += __shfl_xor(v, k);
     return v;
 }
-__device__ __forceinline__ float wave_max(float v)
+template <int G> __device__ __forceinline__ float group_max(float v)
 {
-    for (int k = 32; k; k /= 2) v = fmaxf(v, __shfl_xor(v, k));
+#pragma unroll
+    for (int k = G / 2; k; k /= 2) v = fmaxf(v, __shfl_xor(v, k));
     return v;
 }
 
-// One wave; the lists are complete for the whole block after its next barrier.
-__device__ __forceinline__ void read_entries(const DistillArgs &q, long long row, Entries &e, unsigned *bits)
+// What a row's entries come to: their probabilities' sum, sum p log p, and what the teacher has left.
+struct Mass { double mass, ent, rest; bool some; };
+
+// G lanes, C entries each: action, teacher's logit -> probability p and log p.  An absent entry has action -1 and p = 0.
+template <int G, int C>
+__device__ __forceinline__ Mass weigh(const DistillArgs &q, long long row, const int (&index)[C], const float (&t)[C], double (&p)[C])
 {
-    const int lane = threadIdx.x % 64;
     const double inv_tau = 1.0 / (double)q.tau;
-    bool some = false;
-    double top = -HUGE_VAL;
-    for (int k = lane; k < q.K; k += 64) {
-        const int j = entry_at(q, row * q.K + k);
-        const double t = j >= 0 ? (double)teacher_at(q, row * q.K + k) * inv_tau : -HUGE_VAL;
-        e.index[k] = j, e.p[k] = t;
-        some |= j >= 0;
-        top = t > top || t != t ? t : top;
-        if (bits && j >= 0) atomicOr(&bits[j / 32], 1u << (j % 32));
+    float top = -HUGE_VALF;
+    bool any = false;
+#pragma unroll
+    for (int i = 0; i < C; i++) {
+        top = fmaxf(top, t[i]);
+        any |= index[i] >= 0;
     }
-    for (int k = 32; k; k /= 2) {
-        const double o = __shfl_xor(top, k);
-        top = o > top || o != o ? o : top;
+    Mass e;
+    e.some = group_max<G>(any ? 1.0f : 0.0f) != 0.0f;
+    double logp[C], sum = 0;
+    if (q.lse) {
+        const double lse = q.lse[row];
+#pragma unroll
+        for (int i = 0; i < C; i++) logp[i] = (double)t[i] * inv_tau - lse;
+    } else {
+        top = group_max<G>(top);
+#pragma unroll
+        for (int i = 0; i < C; i++) logp[i] = ((double)t[i] - (double)top) * inv_tau;
     }
-    e.some = __any(some);
-    if (q.lse) top = (double)q.lse[row];
-    double z = 0, sum = 0;
-    if (!q.lse) {
-        for (int k = lane; k < q.K; k += 64) z += e.p[k] == -HUGE_VAL ? 0.0 : exp(e.p[k] - top);
-        z = wave_sum(z);
-    }
-    const double logz = q.lse ? 0.0 : log(z), inv_z = q.lse ? 1.0 : 1.0 / z;
+#pragma unroll
+    for (int i = 0; i < C; i++) p[i] = t[i] == -HUGE_VALF ? 0.0 : exp(logp[i]), sum += p[i];
+    sum = group_sum<G>(sum);
+    const double norm = q.lse ? 1.0 : 1.0 / sum, shift = q.lse ? 0.0 : log(sum);
     double ent = 0;
-    for (int k = lane; k < q.K; k += 64) {
-        const bool none = e.p[k] == -HUGE_VAL;
-        const double u = e.p[k] - top, p = none ? 0.0 : exp(u) * inv_z;
-        e.p[k] = p;
-        sum += p;
-        if (!(p == 0)) ent += p * (u - logz);
+#pragma unroll
+    for (int i = 0; i < C; i++) {
+        if (p[i] == 0) continue;
+        p[i] *= norm;
+        ent += p[i] * (logp[i] - shift);
     }
-    e.mass = wave_sum(sum);
-    e.ent = wave_sum(ent);
-    e.rest = q.lse ? fmax(1.0 - e.mass, 0.0) : 0.0;
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    for (int k = lane; k < q.K; k += 64) {   // an action that several entries name gets the sum, in the order of the entries
-        const int j = e.index[k];
-        double tot = 0;
-        bool first = j >= 0;
-        for (int i = 0; i < q.K; i++)
-            if (e.index[i] == j) {
-                tot += e.p[i];
-                if (i < k) first = false;
-            }
-        e.total[k] = first ? tot : -1.0;
-    }
+    e.ent = group_sum<G>(ent);
+    e.mass = q.lse ? sum : sum > 0 || sum != sum ? sum * norm : 0.0;
+    e.rest = q.lse ? fmax(1.0 - sum, 0.0) : 0.0;
+    if (sum != sum) e.rest = sum;
+    return e;
 }
 
-// One block per row.  The row's packs of 16 bytes stay in registers between the passes where NP of them per thread hold it
-// (KEEP); otherwise each pass reads it again.  MODE 0: loss and statistics, 1: loss and gradient, 2: gradient from the
-// statistics of an earlier loss pass.
-template <typename T, int THREADS, int NP, bool KEEP, int MODE>
-__global__ __launch_bounds__(THREADS) void k_distill_row(DistillArgs q, float c_hi, float c_lo)
+// exp(d / tau) as exp2 of the product with c = log2(e) / tau.  d = z - m is at most 0, so c's rounding is a change of the
+// temperature by 2^-25 of itself, and a -inf logit stays at 0.
+__device__ __forceinline__ float expo(float d, float c) { return __builtin_amdgcn_exp2f(d * c); }
+
+__device__ __forceinline__ double divergence(const Mass &e, double cross, double dsum, double dtail)
 {
-    constexpr int E = 16 / sizeof(T), NW = THREADS / 64;
+    double kl = e.ent - cross;
+    if (!(e.rest == 0)) kl += e.rest * (log(e.rest) - log(dtail) + log(dsum));
+    return kl;
+}
+
+// Small action sets: G lanes of a wave hold a row, E actions and 4 entries a lane, all of it in registers.  MODE 0: loss and
+// statistics, 1: loss and gradient, 2: gradient from the statistics of an earlier loss pass.
+template <typename T, int G, int E, int MODE>
+__global__ __launch_bounds__(256) void k_distill_group(DistillArgs q, float c)
+{
+    constexpr int C = 4;
+    const int lane = threadIdx.x % G;
+    const long long row = (long long)blockIdx.x * (256 / G) + threadIdx.x / G;
+    if (row >= q.R) return;
+    const T *zr = (const T *)q.logits + row * q.ld;
+    T *gr = (T *)q.grad + row * q.V;
+    const float weight = q.weight ? q.weight[row] : 1.0f;
+    const float scale = MODE == 0 ? 0.0f : weight * q.tau * (q.up ? q.up[row] : 1.0f);
+    float z[E], ze[C], t[C];
+    int index[C];
+#pragma unroll
+    for (int i = 0; i < C; i++) {
+        const int k = lane + i * G;
+        index[i] = k < q.K ? entry_at(q, row * q.K + k) : -1;
+        t[i] = index[i] >= 0 ? teacher_at(q, row * q.K + k) : -HUGE_VALF;
+        ze[i] = index[i] >= 0 ? widen(zr[index[i]]) : 0.0f;
+    }
+#pragma unroll
+    for (int i = 0; i < E; i++) {
+        const int j = lane + i * G;
+        z[i] = j < q.V ? widen(zr[j]) : -HUGE_VALF;
+    }
+    double p[C];
+    Mass e = weigh<G, C>(q, row, index, t, p);
+    if (!e.some || (MODE == 2 ? scale == 0.0f || q.stats[row * 4 + 3] == 0.0f : weight == 0.0f)) {   // nothing of the row counts
+        if (MODE != 0)
+#pragma unroll
+            for (int i = 0; i < E; i++) if (lane + i * G < q.V) gr[lane + i * G] = T(0.0f);
+        if (MODE != 2 && lane == 0) {
+            q.loss[row] = 0.0f;
+            if (MODE == 0) q.stats[row * 4 + 3] = 0.0f;
+        }
+        return;
+    }
+    // which of the lane's actions are entries, and what all entries of the same action come to
+    unsigned inside = 0;
+    double total[C];
+    bool first[C];
+#pragma unroll
+    for (int i = 0; i < C; i++) total[i] = 0, first[i] = index[i] >= 0;
+    if (MODE != 0 || q.lse) {
+#pragma unroll
+        for (int i = 0; i < C; i++)
+            for (int l = 0; l < G; l++) {
+                if (l + i * G >= q.K) break;
+                const int j = __shfl(index[i], l, G);
+                if (j >= 0 && j % G == lane) inside |= 1u << (j / G);
+                if (MODE != 0) {
+                    const double pj = __shfl(p[i], l, G);
+#pragma unroll
+                    for (int c = 0; c < C; c++) {
+                        total[c] += index[c] == j ? pj : 0.0;
+                        if (index[c] == j && l + i * G < lane + c * G) first[c] = false;
+                    }
+                }
+            }
+    }
+    float m;
+    double dsum, dtail;
+    if (MODE != 2) {
+        m = -HUGE_VALF;
+#pragma unroll
+        for (int i = 0; i < E; i++) m = fmaxf(m, z[i]);
+        m = group_max<G>(m);
+        float sum = 0, tail = 0;
+#pragma unroll
+        for (int i = 0; i < E; i++) {
+            const float x = expo(z[i] - m, c);
+            sum += x;
+            if (q.lse && !(inside >> i & 1)) tail += x;
+        }
+        dsum = group_sum<G>(sum), dtail = group_sum<G>(tail);
+        if (dtail == 0) e.rest = 0;   // no action outside the entries has anything left
+        const double lsum = log(dsum), inv_tau = 1.0 / (double)q.tau;
+        double cross = 0;
+#pragma unroll
+        for (int i = 0; i < C; i++)
+            if (!(p[i] == 0)) cross += p[i] * (((double)ze[i] - (double)m) * inv_tau - lsum);
+        cross = group_sum<G>(cross);
+        if (lane == 0) {
+            q.loss[row] = (float)((double)weight * q.tau * q.tau * divergence(e, cross, dsum, dtail));
+            if (MODE == 0) *(float4 *)(q.stats + row * 4) = make_float4(m, (float)dsum, (float)dtail, 1.0f);
+        }
+    } else {
+        const float4 st = *(const float4 *)(q.stats + row * 4);
+        m = st.x, dsum = st.y, dtail = st.z;
+        if (dtail == 0) e.rest = 0;
+    }
+    if (MODE == 0) return;
+    const double whole = e.mass + e.rest, outside = e.rest == 0 ? whole : whole - e.rest * dsum / dtail;
+    const float f = (float)(outside / dsum * scale), fi = (float)(whole / dsum * scale);
+#pragma unroll
+    for (int i = 0; i < E; i++) {
+        const int j = lane + i * G;
+        if (j < q.V && !(inside >> i & 1)) gr[j] = narrow<T>(expo(z[i] - m, c) * f);
+    }
+#pragma unroll
+    for (int i = 0; i < C; i++)
+        if (first[i]) gr[index[i]] = narrow<T>(__builtin_fmaf(expo(ze[i] - m, c), fi, -(float)(total[i] * scale)));
+}
+
+// A pack of 16 bytes as it lies in memory.
+struct alignas(16) Raw {
+    unsigned w[4];
+    template <typename P> __device__ __forceinline__ P as() const
+    {
+        P v;
+        __builtin_memcpy(&v, w, 16);
+        return v;
+    }
+    __device__ __forceinline__ void fill(unsigned u) { w[0] = w[1] = w[2] = w[3] = u; }
+};
+template <typename T> __device__ __forceinline__ unsigned lowest_bits();   // a register of -inf
+template <> __device__ __forceinline__ unsigned lowest_bits<float>() { return 0xff800000u; }
+template <> __device__ __forceinline__ unsigned lowest_bits<__bf16>() { return 0xff80ff80u; }
+template <> __device__ __forceinline__ unsigned lowest_bits<_Float16>() { return 0xfc00fc00u; }
+
+// Wide action sets: one block per row.  A row is a run of whole packs, aligned in memory, between two edges of less than a
+// pack, which the block's last two threads take element by element.  The sums take one pass over the row, four packs of a
+// thread on their way at a time, with a running maximum per thread; the gradient takes another, which in the loss and
+// gradient pass finds the row in cache.
+template <typename T, int THREADS, int MODE>
+__global__ __launch_bounds__(THREADS) void k_distill_row(DistillArgs q, float c)
+{
+    constexpr int E = 16 / sizeof(T), NW = THREADS / 64, U = 2;
     using P = Pack<T, E>;
     extern __shared__ double lds[];
-    __shared__ double red[3][NW];
-    __shared__ double share[4];
-    Entries e;
-    e.p = lds, e.total = lds + q.K, e.index = (int *)(lds + 2 * q.K);
-    unsigned *bits = q.lse && MODE != 2 ? (unsigned *)(e.index + q.K) : nullptr;
+    __shared__ double red[2][NW];
+    __shared__ float red_m[NW];
+    __shared__ double share[3];
+    __shared__ int share_some, repeated;
+    double *ep = lds;                                     // [K] probability of an entry
+    float *ez = (float *)(lds + q.K);                     // [K] the student's logit of its action
+    int *ei = (int *)(ez + q.K);                          // [K] its action, -1: absent
+    unsigned *bits = q.lse && MODE != 2 ? (unsigned *)(ei + q.K) : nullptr;   // the entries' actions, E bits a pack
     const long long row = blockIdx.x;
     const T *z = (const T *)q.logits + row * q.ld;
-    T *g = q.grad ? (T *)q.grad + row * q.V : nullptr;
-    const int tid = threadIdx.x, w = tid / 64;
-    // packs are aligned in memory: the first one begins up to E - 1 elements in front of the row
+    T *g = MODE ? (T *)q.grad + row * q.V : nullptr;
+    const int tid = threadIdx.x, w = tid / 64, lane = tid % 64;
+    // pack i covers actions i * E - shift ..; whole packs are [first, last)
     const int shift = (int)(((uintptr_t)z / sizeof(T)) % E);
-    const bool same = g && (int)(((uintptr_t)g / sizeof(T)) % E) == shift;
-    const int n_packs = (q.V + shift + E - 1) / E;
+    const bool same = MODE && (int)(((uintptr_t)g / sizeof(T)) % E) == shift;
+    const int first = shift ? 1 : 0, last = max((q.V + shift) / E, first), n_packs = (q.V + shift + E - 1) / E;
+    // the edges: pack 0 if it is cut, pack `last` if there is one
+    const int edge = tid == THREADS - 1 && shift ? 0 : tid == THREADS - 2 && n_packs > last ? last : -1;
     const float weight = q.weight ? q.weight[row] : 1.0f;
     const float scale = MODE == 0 ? 0.0f : weight * q.tau * (q.up ? q.up[row] : 1.0f);
 
-    auto load = [&](int i, P &v) {
-        const int j = i * E - shift;
-        if (j >= 0 && j + E <= q.V) v = *(const P *)(z + j);
-        else
-#pragma unroll
-            for (int k = 0; k < E; k++) v.v[k] = j + k >= 0 && j + k < q.V ? z[j + k] : T(-HUGE_VALF);
-    };
-    auto store = [&](int i, const P &v) {
-        const int j = i * E - shift;
-        if (same && j >= 0 && j + E <= q.V) *(P *)(g + j) = v;
-        else
-#pragma unroll
-            for (int k = 0; k < E; k++) if (j + k >= 0 && j + k < q.V) g[j + k] = v.v[k];
-    };
-    auto zeros = [&]() {
+    auto load_edge = [&]() {
         P v;
 #pragma unroll
-        for (int k = 0; k < E; k++) v.v[k] = T(0.0f);
-        for (int i = tid; i < n_packs; i += THREADS) store(i, v);
+        for (int k = 0; k < E; k++) {
+            const int j = edge * E - shift + k;
+            v.v[k] = edge >= 0 && j >= 0 && j < q.V ? z[j] : T(-HUGE_VALF);
+        }
+        return v;
+    };
+    auto store_edge = [&](const P &v) {
+#pragma unroll
+        for (int k = 0; k < E; k++) {
+            const int j = edge * E - shift + k;
+            if (edge >= 0 && j >= 0 && j < q.V) g[j] = v.v[k];
+        }
+    };
+    // whole pack i; -inf from `last` on (read where the last one is: nothing is read behind the row)
+    auto load = [&](int i) {
+        Raw r = *(const Raw *)(z + (long long)min(i, last - 1) * E - shift);
+        if (i >= last) r.fill(lowest_bits<T>());
+        return r;
+    };
+    auto store = [&](int i, const P &v) {
+        T *to = g + (long long)i * E - shift;
+        if (same) *(P *)to = v;
+        else *(Loose<T, E> *)to = *(const Loose<T, E> *)&v;
+    };
+    auto nothing = [&]() {   // of the row counts
+        if (MODE != 0) {
+            P v;
+#pragma unroll
+            for (int k = 0; k < E; k++) v.v[k] = T(0.0f);
+            for (int i = first + tid; i < last; i += THREADS) store(i, v);
+            store_edge(v);
+        }
+        if (MODE != 2 && tid == 0) {
+            q.loss[row] = 0.0f;
+            if (MODE == 0) q.stats[row * 4 + 3] = 0.0f;
+        }
     };
 
-    if (MODE == 2 ? (scale == 0.0f || q.stats[row * 4 + 3] == 0.0f) : weight == 0.0f) {   // nothing of the row counts
-        if (MODE != 0) zeros();
-        if (MODE != 2 && tid == 0) {
-            q.loss[row] = 0.0f;
-            if (MODE == 0) q.stats[row * 4 + 3] = 0.0f;
-        }
+    const int start = first + tid;
+    const bool inner = last > first;
+    Raw r[U];
+    auto begin = [&]() {
+        if (inner)
+#pragma unroll
+            for (int u = 0; u < U; u++) r[u] = load(start + u * THREADS);
+    };
+    if (MODE == 2 ? (scale == 0.0f || q.stats[row * 4 + 3] == 0.0f) : weight == 0.0f) {
+        nothing();
         return;
     }
-    P keep[KEEP ? NP : 1];
-    float m = -HUGE_VALF;
-    if (KEEP)
-#pragma unroll
-        for (int n = 0; n < NP; n++) load(tid + n * THREADS, keep[n]);   // -inf behind the row
     if (bits) {
-        for (int i = tid; i < (q.V + 31) / 32; i += THREADS) bits[i] = 0;
+        for (int i = tid; i < (n_packs * E + 31) / 32; i += THREADS) bits[i] = 0;
         __syncthreads();
     }
-    if (w == 0) {
-        read_entries(q, row, e, bits);
-        if (tid == 0) share[0] = e.mass, share[1] = e.ent, share[2] = e.rest, share[3] = e.some ? 1.0 : 0.0;
-    }
-    double dsum = 0, dtail = 0;
-    if (MODE != 2) {
-        if (KEEP)
-#pragma unroll
-            for (int n = 0; n < NP; n++)
-#pragma unroll
-                for (int k = 0; k < E; k++) m = fmaxf(m, widen(keep[n].v[k]));
-        else
-            for (int i = tid; i < n_packs; i += THREADS) {
-                P v;
-                load(i, v);
-#pragma unroll
-                for (int k = 0; k < E; k++) m = fmaxf(m, widen(v.v[k]));
+    if (w == 0) {   // the first wave weighs the entries
+        if (lane == 0) repeated = 0;
+        auto put = [&](int k, int j) {
+            ei[k] = j, ez[k] = j >= 0 ? widen(z[j]) : 0.0f;
+            if (bits && j >= 0) atomicOr(&bits[(j + shift) / 32], 1u << ((j + shift) % 32));
+        };
+        if (q.K <= 64) {
+            int index[1] = {lane < q.K ? entry_at(q, row * q.K + lane) : -1};
+            float t[1] = {index[0] >= 0 ? teacher_at(q, row * q.K + lane) : -HUGE_VALF};
+            double p[1];
+            if (lane < q.K) put(lane, index[0]);
+            const Mass e = weigh<64, 1>(q, row, index, t, p);
+            if (lane < q.K) ep[lane] = p[0];
+            if (lane == 0) share[0] = e.mass, share[1] = e.ent, share[2] = e.rest, share_some = e.some;
+        } else {   // in rounds of 64, over lists in LDS
+            const double inv_tau = 1.0 / (double)q.tau;
+            float top = -HUGE_VALF;
+            bool some = false;
+            for (int k = lane; k < q.K; k += 64) {
+                const int j = entry_at(q, row * q.K + k);
+                const float t = j >= 0 ? teacher_at(q, row * q.K + k) : -HUGE_VALF;
+                put(k, j);
+                ep[k] = t;
+                some |= j >= 0;
+                top = fmaxf(top, t);
             }
-        m = wave_max(m);
-        if (tid % 64 == 0) red[0][w] = m;
-    }
-    __syncthreads();
-    if (MODE != 2) {
-#pragma unroll
-        for (int i = 0; i < NW; i++) m = fmaxf(m, (float)red[0][i]);
-    } else m = q.stats[row * 4];
-    e.mass = share[0], e.ent = share[1], e.rest = share[2], e.some = share[3] != 0.0;
-    if (!e.some) {
-        if (MODE != 0) zeros();
-        if (MODE != 2 && tid == 0) {
-            q.loss[row] = 0.0f;
-            if (MODE == 0) q.stats[row * 4 + 3] = 0.0f;
+            const double from = q.lse ? (double)q.lse[row] : (double)group_max<64>(top) * inv_tau;
+            double total = 0, ent = 0;
+            for (int k = lane; k < q.K; k += 64) total += ep[k] == -HUGE_VAL ? 0.0 : exp(ep[k] * inv_tau - from);
+            total = group_sum<64>(total);
+            const double norm = q.lse ? 1.0 : 1.0 / total, less = q.lse ? 0.0 : log(total);
+            for (int k = lane; k < q.K; k += 64) {
+                const double u = ep[k] * inv_tau - from, x = ep[k] == -HUGE_VAL ? 0.0 : exp(u) * norm;
+                ep[k] = x;
+                if (!(x == 0)) ent += x * (u - less);
+            }
+            ent = group_sum<64>(ent);
+            some = __any(some);
+            if (lane == 0) {
+                share[0] = q.lse ? total : total == 0 ? 0.0 : total * norm, share[1] = ent;
+                share[2] = q.lse ? (total != total ? total : fmax(1.0 - total, 0.0)) : 0.0;
+                share_some = some;
+            }
         }
+        begin();
+    } else begin();   // the other waves' first packs are on their way meanwhile
+    float m = -HUGE_VALF, sum = 0, tail = 0;
+    // adds a pack's exponentials to the sums
+    auto add = [&](int i, const P &v) {
+        float x[E], s = 0;
+#pragma unroll
+        for (int k = 0; k < E; k++) x[k] = expo(widen(v.v[k]) - m, c), s += x[k];
+        sum += s;
+        if (bits && i < n_packs) {
+            const unsigned in = E == 8 ? ((const uint8_t *)bits)[i] : ((const uint8_t *)bits)[i / 2] >> (i % 2 * 4) & 15;
+            if (in) {
+                s = 0;
+#pragma unroll
+                for (int k = 0; k < E; k++) s += in >> k & 1 ? 0.0f : x[k];
+            }
+            tail += s;
+        }
+    };
+    auto top_of = [&](const P &v) {
+        float t = widen(v.v[0]);
+#pragma unroll
+        for (int k = 1; k < E; k++) t = fmaxf(t, widen(v.v[k]));
+        return t;
+    };
+    __syncthreads();
+    Mass e{share[0], share[1], share[2], share_some != 0};
+    if (!e.some) {
+        nothing();
         return;
     }
-    // exp((z - m) / tau) as exp2 of the product with log2(e) / tau in two parts (c_lo > 0 keeps a -inf logit at -inf)
-    auto expo = [&](T v) {
-        const float d = widen(v) - m;
-        return __builtin_amdgcn_exp2f(__builtin_fmaf(d, c_lo, d * c_hi));
-    };
+    double dsum, dtail;
     if (MODE != 2) {
-        float sum = 0, tail = 0;
-        auto add = [&](int i, const P &v) {
-            const int j = i * E - shift;
-#pragma unroll
-            for (int k = 0; k < E; k++) {
-                const float x = expo(v.v[k]);
-                sum += x;
-                if (bits && j + k >= 0 && j + k < q.V && !(bits[(j + k) / 32] >> ((j + k) % 32) & 1)) tail += x;
+        // one pass: whenever the thread's maximum rises, what it has summed so far is scaled down to the new one
+        auto take = [&](int i, const P &v) {
+            const float top = top_of(v);
+            if (top > m) {
+                const float down = m == -HUGE_VALF ? 0.0f : expo(m - top, c);
+                sum *= down, tail *= down, m = top;
             }
+            if (m != -HUGE_VALF) add(i, v);
+            else
+#pragma unroll
+                for (int k = 0; k < E; k++) if (v.v[k] != v.v[k]) sum = tail = widen(v.v[k]);   // not a number among nothing but -inf
         };
-        if (KEEP)
+        if (inner)
+            for (int i = start;;) {
+                const int next = i + U * THREADS;
+                Raw ahead[U];
+                if (next < last)
 #pragma unroll
-            for (int n = 0; n < NP; n++) add(tid + n * THREADS, keep[n]);
-        else
-            for (int i = tid; i < n_packs; i += THREADS) {
-                P v;
-                load(i, v);
-                add(i, v);
+                    for (int u = 0; u < U; u++) ahead[u] = load(next + u * THREADS);
+#pragma unroll
+                for (int u = 0; u < U; u++) take(i + u * THREADS, r[u].template as<P>());
+                if (next >= last) break;
+                i = next;
+#pragma unroll
+                for (int u = 0; u < U; u++) r[u] = ahead[u];
             }
-        dsum = wave_sum(sum), dtail = wave_sum(tail);
-        if (tid % 64 == 0) red[1][w] = dsum, red[2][w] = dtail;
+        if (edge >= 0) take(edge, load_edge());
+        const float own = m;
+        m = group_max<64>(m);
+        if (lane == 0) red_m[w] = m;
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < NW; i++) m = fmaxf(m, red_m[i]);
+        const float down = own == -HUGE_VALF ? 1.0f : expo(own - m, c);
+        sum *= down, tail *= down;
+        if (m == -HUGE_VALF) sum = tail = m - m;   // no logit above -inf: not a number
+        dsum = group_sum<64>(sum), dtail = group_sum<64>(tail);
+        if (lane == 0) red[0][w] = dsum, red[1][w] = dtail;
         __syncthreads();
         dsum = dtail = 0;
 #pragma unroll
-        for (int i = 0; i < NW; i++) dsum += red[1][i], dtail += red[2][i];
-        if (!(dtail != 0)) e.rest = 0;   // no action outside the entries has anything left
-        if (w == 0) {
+        for (int i = 0; i < NW; i++) dsum += red[0][i], dtail += red[1][i];
+        if (dtail == 0) e.rest = 0;   // no action outside the entries has anything left
+        if (w == NW - 1) {
             double cross = 0;
             const double lsum = log(dsum), inv_tau = 1.0 / (double)q.tau;
-            for (int k = tid; k < q.K; k += 64)
-                if (e.index[k] >= 0 && !(e.p[k] == 0))
-                    cross += e.p[k] * (((double)widen(z[e.index[k]]) - (double)m) * inv_tau - lsum);
-            cross = wave_sum(cross);
-            if (tid == 0) {
-                double kl = e.ent - cross;
-                if (!(e.rest == 0)) kl += e.rest * (log(e.rest) - log(dtail) + lsum);
-                q.loss[row] = (float)((double)weight * q.tau * q.tau * kl);
-                if (MODE == 0) {
-                    float *st = q.stats + row * 4;
-                    st[0] = m, st[1] = (float)dsum, st[2] = (float)dtail, st[3] = 1.0f;
-                }
+            for (int k = lane; k < q.K; k += 64)
+                if (!(ep[k] == 0)) cross += ep[k] * (((double)ez[k] - (double)m) * inv_tau - lsum);
+            cross = group_sum<64>(cross);
+            if (lane == 0) {
+                q.loss[row] = (float)((double)weight * q.tau * q.tau * divergence(e, cross, dsum, dtail));
+                if (MODE == 0) *(float4 *)(q.stats + row * 4) = make_float4(m, (float)dsum, (float)dtail, 1.0f);
             }
         }
     } else {
-        dsum = q.stats[row * 4 + 1], dtail = q.stats[row * 4 + 2];
-        if (!(dtail != 0)) e.rest = 0;
+        const float4 st = *(const float4 *)(q.stats + row * 4);
+        m = st.x, dsum = st.y, dtail = st.z;
+        if (dtail == 0) e.rest = 0;
     }
     if (MODE == 0) return;
     // q_j times what stands outside the entries; the entries themselves are put right behind the barrier
-    const double whole = e.mass + e.rest;
-    const double outside = e.rest == 0 ? whole : whole - e.rest * dsum / dtail;
-    const float f = (float)(outside / dsum * scale);
-    auto emit = [&](int i, const P &v) {
+    const double whole = e.mass + e.rest, outside = e.rest == 0 ? whole : whole - e.rest * dsum / dtail;
+    const float f = (float)(outside / dsum * scale), fi = (float)(whole / dsum * scale);
+    for (int k = tid; k < q.K; k += THREADS) {
+        bool other = false;
+        for (int i = 0; i < q.K; i++) other |= i != k && ei[i] == ei[k];
+        if (other && ei[k] >= 0) repeated = 1;
+    }
+    auto emit = [&](const P &v) {
         P o;
 #pragma unroll
-        for (int k = 0; k < E; k++) o.v[k] = narrow<T>(expo(v.v[k]) * f);
-        store(i, o);
+        for (int k = 0; k < E; k++) o.v[k] = narrow<T>(expo(widen(v.v[k]) - m, c) * f);
+        return o;
     };
-    if (KEEP)
+    if (inner)
+        for (int i = start; i < last; i += U * THREADS) {
+            if (MODE == 1 || i != start)
 #pragma unroll
-        for (int n = 0; n < NP; n++) {
-            if (tid + n * THREADS < n_packs) emit(tid + n * THREADS, keep[n]);
+                for (int u = 0; u < U; u++) r[u] = load(i + u * THREADS);
+#pragma unroll
+            for (int u = 0; u < U; u++) if (i + u * THREADS < last) store(i + u * THREADS, emit(r[u].template as<P>()));
         }
-    else
-        for (int i = tid; i < n_packs; i += THREADS) {
-            P v;
-            load(i, v);
-            emit(i, v);
-        }
+    if (edge >= 0) store_edge(emit(load_edge()));
     __syncthreads();
     for (int k = tid; k < q.K; k += THREADS) {
-        const double tot = e.total[k];
-        const int j = e.index[k];
-        if (j >= 0 && !(tot < 0)) g[j] = narrow<T>((float)(((double)expo(z[j]) / dsum * whole - tot) * scale));
+        const int j = ei[k];
+        if (j < 0) continue;
+        double total = ep[k];
+        bool lead = true;
+        if (repeated) {   // an action that several entries name gets the sum, in the order of the entries
+            total = 0;
+            for (int i = 0; i < q.K; i++)
+                if (ei[i] == j) {
+                    total += ep[i];
+                    lead &= i >= k;
+                }
+        }
+        if (lead) g[j] = narrow<T>(__builtin_fmaf(expo(ez[k] - m, c), fi, -(float)(total * scale)));
     }
 }
 

@@ -18,21 +18,21 @@ static size_t size_of(int type) { return type == MZ_F64 ? 8 : type == MZ_F32 ? 4
 // ------------------------------------------------------------------------------------------------ recurrence
 
 // Positions a strand holds in registers; below REC_FEW_TILES channel tiles the axis is cut into segments.
-constexpr int REC_LENGTH(int size, bool backward) { return size == 8 ? 8 : backward ? 8 : 16; }
+constexpr int REC_LENGTH = 8;
 constexpr long long REC_FEW_TILES = 128, REC_WANT_BLOCKS = 512, REC_MAX_SEGMENTS = 64;
 
 // How a recurrence is run: chosen by sizes, strides and alignment alone, for the workspace query and the call alike.
 struct RecurrencePlan {
     bool channels, brief;    // channels contiguous; so few positions that a thread walks them all
-    int vec;                 // channels a thread holds
+    int vec, lanes;          // channels a thread holds, lanes of a strand
     int strands, segments;
     long long segment;
 };
 
 // VEC = 2 is a 4-byte access of a 16-bit type
-static RecurrencePlan plan_recurrence(const mz_recurrence *a, bool backward)
+static RecurrencePlan plan_recurrence(const mz_recurrence *a)
 {
-    RecurrencePlan p{true, false, 1, REC_STRANDS, 1, a->T};
+    RecurrencePlan p{true, false, 1, 32, 1, 1, a->T};
     uint64_t low = 0;   // low bits of every address and step along the axis and the sequences
     const int size = (int)size_of(a->type);
     for (const mz_strided *t : {&a->gate, &a->x, &a->out, &a->y, &a->out_gate}) {
@@ -51,27 +51,34 @@ static RecurrencePlan plan_recurrence(const mz_recurrence *a, bool backward)
         return p;
     }
     p.vec = size == 2 && fits(2) ? 2 : 1;
-    const int L = REC_LENGTH(size, backward);
-    const long long tiles = (long long)a->B * ((a->D + REC_LANES * p.vec - 1) / (REC_LANES * p.vec));
-    p.strands = (int)std::min<long long>(REC_STRANDS, std::max<long long>(2, (a->T + L - 1) / L));
+    auto tiles_of = [&](int lanes) { return (long long)a->B * ((a->D + lanes * p.vec - 1) / (lanes * p.vec)); };
+    p.lanes = tiles_of(64) >= REC_WANT_BLOCKS || tiles_of(32) < REC_FEW_TILES ? 64 : 32;
+    const long long tiles = tiles_of(p.lanes);
+    const int most = REC_THREADS / p.lanes;
+    p.strands = (int)std::min<long long>(most, std::max<long long>(2, (a->T + REC_LENGTH - 1) / REC_LENGTH));
     if (tiles < REC_FEW_TILES) {
-        const long long rounds = (a->T + (long long)REC_STRANDS * L - 1) / (REC_STRANDS * L);
+        const long long rounds = (a->T + (long long)most * REC_LENGTH - 1) / (most * REC_LENGTH);
         const long long want = std::min<long long>({rounds / 2, (REC_WANT_BLOCKS + tiles - 1) / tiles, REC_MAX_SEGMENTS});
         if (want > 1) {
-            p.segment = (rounds + want - 1) / want * REC_STRANDS * L;
+            p.segment = (rounds + want - 1) / want * most * REC_LENGTH;
             p.segments = (int)((a->T + p.segment - 1) / p.segment);
         }
     }
     return p;
 }
 
+template <typename T, int VEC, int LANES, bool BWD> static void launch_channels(const RecurrencePlan &p, const RecurrenceArgs &q, hipStream_t st)
+{
+    const unsigned tiles = (unsigned)((long long)q.B * ((q.D + LANES * VEC - 1) / (LANES * VEC)));
+    if (q.segments > 1)
+        hipLaunchKernelGGL((k_recurrence_maps<T, VEC, LANES, REC_LENGTH, BWD>), dim3(tiles, q.segments - 1), dim3(REC_THREADS), 0, st, q);
+    hipLaunchKernelGGL((k_recurrence_channels<T, VEC, LANES, REC_LENGTH, BWD>), dim3(tiles, q.segments), dim3(LANES * p.strands), 0, st, q);
+}
+
 template <typename T, int VEC, bool BWD> static void launch_channels(const RecurrencePlan &p, const RecurrenceArgs &q, hipStream_t st)
 {
-    constexpr int L = REC_LENGTH((int)sizeof(T), BWD);
-    const unsigned tiles = (unsigned)((long long)q.B * ((q.D + REC_LANES * VEC - 1) / (REC_LANES * VEC)));
-    if (q.segments > 1)
-        hipLaunchKernelGGL((k_recurrence_maps<T, VEC, L, BWD>), dim3(tiles, q.segments - 1), dim3(REC_LANES * REC_STRANDS), 0, st, q);
-    hipLaunchKernelGGL((k_recurrence_channels<T, VEC, L, BWD>), dim3(tiles, q.segments), dim3(REC_LANES * p.strands), 0, st, q);
+    if (p.lanes == 64) launch_channels<T, VEC, 64, BWD>(p, q, st);
+    else launch_channels<T, VEC, 32, BWD>(p, q, st);
 }
 
 template <typename T, int VEC, bool BWD> static void launch_short(const RecurrenceArgs &q, hipStream_t st)
@@ -122,7 +129,7 @@ template <bool BWD> static int run_recurrence(const mz_recurrence *a, void *stre
 {
     (void)hipGetLastError();
     if (int rc = check_recurrence(a, BWD, fn)) return rc;
-    const RecurrencePlan p = plan_recurrence(a, BWD);
+    const RecurrencePlan p = plan_recurrence(a);
     if (a->workspace_bytes < (int64_t)maps_bytes(a, p) || (p.segments > 1 && !a->workspace))
         return api_fail(MZ_ERR_ARG, std::string(fn) + ": the workspace is smaller than mz_linear_recurrence_workspace says");
     RecurrenceArgs q{};
@@ -161,24 +168,38 @@ extern "C" int mz_linear_recurrence_workspace(const mz_recurrence *args_h, int32
 {
     if (int rc = check_recurrence(args_h, backward != 0, "mz_linear_recurrence_workspace")) return rc;
     if (!out_bytes) return api_fail(MZ_ERR_ARG, "mz_linear_recurrence_workspace: null argument");
-    *out_bytes = (int64_t)maps_bytes(args_h, plan_recurrence(args_h, backward != 0));
+    *out_bytes = (int64_t)maps_bytes(args_h, plan_recurrence(args_h));
     return MZ_OK;
 }
 
 // ------------------------------------------------------------------------------------------------ distillation
 
-template <typename T, int THREADS, int NP, bool KEEP, int MODE>
-static void launch_distill(const DistillArgs &q, float c_hi, float c_lo, hipStream_t st)
+template <typename T, int G, int E, int MODE> static void launch_group(const DistillArgs &q, float c, hipStream_t st)
 {
-    const size_t lds = (size_t)q.K * (8 + 8 + 4) + (q.lse && MODE != 2 ? 4 * (((size_t)q.V + 31) / 32) : 0);
-    hipLaunchKernelGGL((k_distill_row<T, THREADS, NP, KEEP, MODE>), dim3((unsigned)q.R), dim3(THREADS), lds, st, q, c_hi, c_lo);
+    constexpr int rows = 256 / G;
+    hipLaunchKernelGGL((k_distill_group<T, G, E, MODE>), dim3((unsigned)(((long long)q.R + rows - 1) / rows)), dim3(256), 0, st, q, c);
 }
 
-template <typename T, int MODE> static void launch_distill(const DistillArgs &q, float c_hi, float c_lo, hipStream_t st)
+constexpr int P64 = 512, P128 = 1024, P256 = 2048, P512 = 8192;
+template <typename T, int THREADS, int MODE> static void launch_row(const DistillArgs &q, float c, hipStream_t st)
 {
-    if (q.V <= 2048) launch_distill<T, 64, 1, false, MODE>(q, c_hi, c_lo, st);
-    else if (q.V <= 16384) launch_distill<T, 256, 1, false, MODE>(q, c_hi, c_lo, st);
-    else launch_distill<T, 1024, 1, false, MODE>(q, c_hi, c_lo, st);
+    const size_t lds = (size_t)q.K * (8 + 4 + 4) + (q.lse && MODE != 2 ? 4 * (((size_t)q.V + 8 + 31) / 32) : 0);
+    hipLaunchKernelGGL((k_distill_row<T, THREADS, MODE>), dim3((unsigned)q.R), dim3(THREADS), lds, st, q, c);
+}
+
+template <typename T, int MODE> static void launch_distill(const DistillArgs &q, float c, hipStream_t st)
+{
+    constexpr int W = 16 / (int)sizeof(T);   // actions of a pack
+    const int packs = (q.V + W - 1) / W + 1;   // one more where a row begins inside a pack
+    if (q.V <= 16 && q.K <= 16) launch_group<T, 4, 4, MODE>(q, c, st);
+    else if (q.V <= 64 && q.K <= 64) launch_group<T, 16, 4, MODE>(q, c, st);
+    else if (q.V <= 256 && q.K <= 64) launch_group<T, 64, 4, MODE>(q, c, st);
+    else if (q.V <= 1024 && q.K <= 64) launch_group<T, 64, 16, MODE>(q, c, st);
+    else if (packs <= P64) launch_row<T, 64, MODE>(q, c, st);
+    else if (packs <= P128) launch_row<T, 128, MODE>(q, c, st);
+    else if (packs <= P256) launch_row<T, 256, MODE>(q, c, st);
+    else if (packs <= P512) launch_row<T, 512, MODE>(q, c, st);
+    else launch_row<T, 1024, MODE>(q, c, st);
 }
 
 template <int MODE> static int run_distill(const mz_distill *a, void *stream, const char *fn)
@@ -197,16 +218,12 @@ template <int MODE> static int run_distill(const mz_distill *a, void *stream, co
     q.logits = a->logits, q.ld = a->logits_stride, q.index = a->index, q.teacher = a->teacher, q.lse = a->lse, q.weight = a->weight;
     q.up = MODE == 2 ? a->grad_loss : nullptr, q.loss = a->loss, q.grad = MODE ? a->grad : nullptr, q.stats = a->stats;
     q.R = a->R, q.V = a->V, q.K = a->K, q.index64 = a->index64, q.teacher_type = a->teacher_type, q.tau = a->temperature;
-    // log2(e) / tau = c_hi + c_lo, c_hi rounded towards zero and c_lo kept above zero
-    const double c = 1.4426950408889634074 / (double)a->temperature;
-    float c_hi = (float)c;
-    if ((double)c_hi > c) c_hi = std::nextafter(c_hi, 0.0f);
-    const float c_lo = std::fmax((float)(c - (double)c_hi), 1e-30f);
+    const float c = (float)(1.4426950408889634074 / (double)a->temperature);   // log2(e) / temperature
     hipStream_t st = (hipStream_t)stream;
     switch (a->type) {
-    case MZ_F32: launch_distill<float, MODE>(q, c_hi, c_lo, st); break;
-    case MZ_BF16: launch_distill<__bf16, MODE>(q, c_hi, c_lo, st); break;
-    default: launch_distill<_Float16, MODE>(q, c_hi, c_lo, st);
+    case MZ_F32: launch_distill<float, MODE>(q, c, st); break;
+    case MZ_BF16: launch_distill<__bf16, MODE>(q, c, st); break;
+    default: launch_distill<_Float16, MODE>(q, c, st);
     }
     return api_launch_status(fn);
 }

@@ -81,26 +81,35 @@ template <typename T, int VEC, int L, bool BWD> struct Strand {
     }
 };
 
-constexpr int REC_LANES = 32, REC_STRANDS = 16;   // lanes along the channels, strands of a block
+// Neighbouring tiles go to the same compute die (workgroups are dealt to the 8 dies in turn), whose cache then holds the lines
+// that tiles share where rows are no multiple of them.
+__device__ __forceinline__ unsigned tile_index()
+{
+    return gridDim.x % 8 ? blockIdx.x : blockIdx.x % 8 * (gridDim.x / 8) + blockIdx.x / 8;
+}
 
-// Channels contiguous: 32 neighbouring lanes hold 32 * VEC neighbouring channels (128 bytes of a position) and walk L
-// consecutive positions in registers; the block's strands follow each other in time and exchange their maps through LDS,
+constexpr int REC_THREADS = 512;   // of a block: strands of 32 or 64 lanes along the channels
+
+// Channels contiguous: LANES neighbouring lanes hold LANES * VEC neighbouring channels (a "strand") and walk L consecutive
+// positions in registers; the block's strands follow each other in time and exchange their maps through LDS,
 // one barrier per round of strands, while the next round's loads are on their way.
 // A grid of few channel tiles leaves compute units idle: the axis is then cut into segments of one block each, whose maps
 // k_recurrence_maps has left in memory; a block folds those of the segments before its own.
-template <typename T, int VEC, int L, bool BWD>
-__global__ __launch_bounds__(REC_LANES * REC_STRANDS) void k_recurrence_channels(RecurrenceArgs q)
+template <typename T, int VEC, int LANES, int L, bool BWD>
+__global__ __launch_bounds__(REC_THREADS) void k_recurrence_channels(RecurrenceArgs q)
 {
+    constexpr int STRANDS = REC_THREADS / LANES;
     using A = acc_t<T>;
     using P = Pack<T, VEC>;
     struct Map { A a[VEC], x[VEC]; };
-    __shared__ Map run[2][REC_STRANDS][REC_LANES];
-    const int nv = blockDim.x / REC_LANES;
-    const int tiles = (q.D + REC_LANES * VEC - 1) / (REC_LANES * VEC);
+    __shared__ Map run[2][STRANDS][LANES];
+    const int nv = blockDim.x / LANES;
+    const int tiles = (q.D + LANES * VEC - 1) / (LANES * VEC);
     // segments of one tile run from the last to the first: what the maps' pass read last is read first
     const int seg = q.segments - 1 - blockIdx.y;
-    const int b = blockIdx.x / tiles, c = threadIdx.x % REC_LANES, v = threadIdx.x / REC_LANES;
-    const int d0 = (blockIdx.x % tiles) * REC_LANES * VEC + c * VEC;
+    const int tile = tile_index();
+    const int b = tile / tiles, c = threadIdx.x % LANES, v = threadIdx.x / LANES;
+    const int d0 = (tile % tiles) * LANES * VEC + c * VEC;
     const bool live = d0 < q.D;
     const int d = live ? d0 : q.D - VEC;   // idle lanes read what the last live one reads
     const long long row = (long long)b * q.D + d;
@@ -181,19 +190,21 @@ __global__ __launch_bounds__(REC_LANES * REC_STRANDS) void k_recurrence_channels
 
 // The maps of all segments but the last: every strand of a block composes a stretch of its own, and the first strand folds
 // the stretches.
-template <typename T, int VEC, int L, bool BWD>
-__global__ __launch_bounds__(REC_LANES * REC_STRANDS) void k_recurrence_maps(RecurrenceArgs q)
+template <typename T, int VEC, int LANES, int L, bool BWD>
+__global__ __launch_bounds__(REC_THREADS) void k_recurrence_maps(RecurrenceArgs q)
 {
+    constexpr int STRANDS = REC_THREADS / LANES;
     using A = acc_t<T>;
     struct Map { A a[VEC], x[VEC]; };
-    __shared__ Map run[REC_STRANDS][REC_LANES];
-    const int tiles = (q.D + REC_LANES * VEC - 1) / (REC_LANES * VEC);
+    __shared__ Map run[STRANDS][LANES];
+    const int tiles = (q.D + LANES * VEC - 1) / (LANES * VEC);
     const int seg = blockIdx.y;
-    const int b = blockIdx.x / tiles, c = threadIdx.x % REC_LANES, v = threadIdx.x / REC_LANES;
-    const int d0 = (blockIdx.x % tiles) * REC_LANES * VEC + c * VEC;
+    const int tile = tile_index();
+    const int b = tile / tiles, c = threadIdx.x % LANES, v = threadIdx.x / LANES;
+    const int d0 = (tile % tiles) * LANES * VEC + c * VEC;
     const bool live = d0 < q.D;
     const int d = live ? d0 : q.D - VEC;
-    const long long stretch = ((q.segment + REC_STRANDS - 1) / REC_STRANDS + L - 1) / L * L;
+    const long long stretch = ((q.segment + STRANDS - 1) / STRANDS + L - 1) / L * L;
     const long long last = (seg + 1) * q.segment;   // below T: the last segment's map is not needed
     const long long begin = min(seg * q.segment + v * stretch, last), end = min(begin + stretch, last);
     Map m;
@@ -214,7 +225,7 @@ __global__ __launch_bounds__(REC_LANES * REC_STRANDS) void k_recurrence_maps(Rec
     run[v][c] = m;
     __syncthreads();
     if (v == 0 && live) {
-        for (int i = 1; i < REC_STRANDS; i++) {
+        for (int i = 1; i < STRANDS; i++) {
             const Map o = run[i][c];
 #pragma unroll
             for (int j = 0; j < VEC; j++) m.x[j] = fma_acc(o.a[j], m.x[j], o.x[j]), m.a[j] *= o.a[j];
