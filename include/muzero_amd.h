@@ -485,6 +485,7 @@ int mz_distill_loss_grad(const mz_distill *args_h, void *stream);
  * mcts/action_selection.py:69).  A draw is the first index whose running sum exceeds u_sample[b] * the whole, in float64.
  * Entries that are negative, infinite or NaN count as 0; a drafted token outside 0..V-1 is not kept; a target row without
  * any mass yields token -1.  out holds the kept drafts, the drawn token, and -1 behind it. */
+#define MZ_VERIFY_MAX_ACTIONS 1048576
 typedef struct mz_verify {
     int32_t type, token64;      /* type of draft and target; 1 = tokens and out are int64, 0 = int32 */
     int32_t B, K, V, reserved;

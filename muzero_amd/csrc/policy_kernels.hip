@@ -234,10 +234,19 @@ extern "C" int mz_distill_grad(const mz_distill *args_h, void *stream) { return 
 
 // ------------------------------------------------------------------------------------------------ verification
 
+template <typename T, int G> static void launch_verify_group(const VerifyArgs &q, hipStream_t st)
+{
+    constexpr int n = 256 / G;
+    hipLaunchKernelGGL((k_verify_group<T, G>), dim3((unsigned)((q.B + (n - 1ll)) / n)), dim3(256), 0, st, q);
+}
+
 template <typename T> static void launch_verify(const VerifyArgs &q, hipStream_t st)
 {
-    const unsigned threads = q.V <= 64 ? 64 : q.V <= 1024 ? 128 : q.V <= 8192 ? 256 : 1024;   // more than one wave above 64 actions
-    hipLaunchKernelGGL((k_verify<T>), dim3((unsigned)q.B), dim3(threads), 0, st, q);
+    if (q.V <= 16) return launch_verify_group<T, 4>(q, st);
+    if (q.V <= 64) return launch_verify_group<T, 16>(q, st);
+    if (q.V <= 256) return launch_verify_group<T, 64>(q, st);
+    const int stretches = (q.V + STRETCH<T> - 1) / STRETCH<T>;
+    hipLaunchKernelGGL((k_verify<T>), dim3((unsigned)q.B), dim3(64 * std::min(stretches, 16)), 8 * (size_t)stretches, st, q);
 }
 
 extern "C" int mz_verify_drafts(const mz_verify *a, void *stream)
@@ -246,7 +255,8 @@ extern "C" int mz_verify_drafts(const mz_verify *a, void *stream)
     (void)hipGetLastError();
     if (!a) return api_fail(MZ_ERR_ARG, std::string(fn) + ": null argument");
     if (a->type < MZ_F32 || a->type > MZ_F64) return api_fail(MZ_ERR_ARG, std::string(fn) + ": unknown element type");
-    if (a->B < 1 || a->K < 0 || a->V < 1) return api_fail(MZ_ERR_ARG, std::string(fn) + ": sizes must be positive");
+    if (a->B < 1 || a->K < 0 || a->K >= INT32_MAX || a->V < 1 || a->V > MZ_VERIFY_MAX_ACTIONS)
+        return api_fail(MZ_ERR_ARG, std::string(fn) + ": sizes must be positive, and at most " + std::to_string(MZ_VERIFY_MAX_ACTIONS) + " actions");
     if (!a->target || !a->u_sample || !a->accepted || !a->out || (a->K && (!a->tokens || !a->u_accept)))
         return api_fail(MZ_ERR_ARG, std::string(fn) + ": null tensor");
     VerifyArgs q{};

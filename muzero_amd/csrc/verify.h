@@ -32,121 +32,248 @@ __device__ __forceinline__ long long drafted(const VerifyArgs &q, long long i)
     return q.token64 ? ((const long long *)q.tokens)[i] : (long long)((const int *)q.tokens)[i];
 }
 
-// How many drafts of sequence b are kept; every thread of the block gets the answer.
-template <typename T> __device__ __forceinline__ int kept(const VerifyArgs &q, int b, int length, int *first)
+__device__ __forceinline__ int length_of(const VerifyArgs &q, long long b)
 {
-    if (threadIdx.x == 0) *first = length;
-    __syncthreads();
-    for (int k = threadIdx.x; k < length; k += blockDim.x) {
-        const long long x = drafted(q, (long long)b * q.K + k);
-        bool ok = false;
-        if (x >= 0 && x < q.V) {
-            const double p = mass_of(((const T *)q.target)[(long long)b * q.target_b + (long long)k * q.target_k + x]);
-            const double d = q.draft ? mass_of(((const T *)q.draft)[(long long)b * q.draft_b + (long long)k * q.draft_k + x]) : 1.0;
-            ok = q.u_accept[(long long)b * q.K + k] * d < p;
-        }
-        if (!ok) atomicMin(first, k);
-    }
-    __syncthreads();
-    return *first;
+    const int n = q.lengths ? q.lengths[b] : q.K;
+    return n < 0 ? 0 : n > q.K ? q.K : n;
 }
 
-// The row to draw from: p, or what p has more than q.
+// Whether draft k of sequence b is kept.
+template <typename T> __device__ __forceinline__ bool passes(const VerifyArgs &q, long long b, int k)
+{
+    const long long x = drafted(q, b * q.K + k);
+    const double u = q.u_accept[b * q.K + k];
+    if (x < 0 || x >= q.V) return false;
+    const double p = mass_of(((const T *)q.target)[b * q.target_b + k * q.target_k + x]);
+    const double d = q.draft ? mass_of(((const T *)q.draft)[b * q.draft_b + k * q.draft_k + x]) : 1.0;
+    return u * d < p;
+}
+
+// The row to draw from once n of `length` drafts are kept: p, or what p has more than the draft's policy.
 template <typename T> struct Left {
     const T *p, *d;
     int only;        // a draft without probabilities: the action that is taken out, else -1
-    __device__ __forceinline__ double at(int j) const
+    __device__ __forceinline__ Left(const VerifyArgs &q, long long b, int n, int length)
+        : p((const T *)q.target + b * q.target_b + n * q.target_k), d(nullptr), only(-1)
     {
-        double v = mass_of(p[j]);
-        if (d) v = fmax(v - mass_of(d[j]), 0.0);
+        if (n >= length) return;
+        if (q.draft) d = (const T *)q.draft + b * q.draft_b + n * q.draft_k;
+        else {
+            const long long x = drafted(q, b * q.K + n);
+            only = x >= 0 && x < q.V ? (int)x : -1;
+        }
+    }
+    __device__ __forceinline__ bool whole() const { return !d && only < 0; }
+    __device__ __forceinline__ double of(T pj, T dj, int j) const
+    {
+        const double v = d ? fmax(mass_of(pj) - mass_of(dj), 0.0) : mass_of(pj);
         return j == only ? 0.0 : v;
     }
 };
 
-__device__ __forceinline__ double block_sum_d(double v, double *red)
+__device__ __forceinline__ void put_token(const VerifyArgs &q, long long b, int n, int k, int token)
 {
-    for (int k = 32; k; k /= 2) v += __shfl_xor(v, k);
-    __syncthreads();
-    if (threadIdx.x % 64 == 0) red[threadIdx.x / 64] = v;
-    __syncthreads();
-    v = 0;
-    for (int i = 0; i < (int)blockDim.x / 64; i++) v += red[i];
+    const long long x = k < n ? drafted(q, b * q.K + k) : k == n ? token : -1;
+    if (q.token64) ((long long *)q.out)[b * (q.K + 1) + k] = x;
+    else ((int *)q.out)[b * (q.K + 1) + k] = (int)x;
+}
+
+template <int G> __device__ __forceinline__ double running_sum(double v, int lane)
+{
+#pragma unroll
+    for (int k = 1; k < G; k *= 2) {
+        const double o = __shfl_up(v, k, G);
+        if (lane >= k) v += o;
+    }
     return v;
 }
 
-// One block per sequence.
+// The lowest lane of the G (a power of two) whose flag is set, or G; and the highest, or -1.
+template <int G> __device__ __forceinline__ int lowest_lane(bool flag)
+{
+    unsigned long long m = __ballot(flag);
+    if (G < 64) m = m >> (threadIdx.x % 64 / G * G) & ((1ull << (G & 63)) - 1);
+    return m ? __ffsll((long long)m) - 1 : G;
+}
+template <int G> __device__ __forceinline__ int highest_lane(bool flag)
+{
+    unsigned long long m = __ballot(flag);
+    if (G < 64) m = m >> (threadIdx.x % 64 / G * G) & ((1ull << (G & 63)) - 1);
+    return m ? 63 - __clzll((long long)m) : -1;
+}
+
+// Small action sets: G lanes of a wave serve a sequence, 4 neighbouring actions a lane, all in registers.
+template <typename T, int G> __global__ __launch_bounds__(256) void k_verify_group(VerifyArgs q)
+{
+    constexpr int E = 4;
+    const int lane = threadIdx.x % G;
+    const long long seq = (long long)blockIdx.x * (256 / G) + threadIdx.x / G;
+    const bool live = seq < q.B;
+    const long long b = live ? seq : q.B - 1;   // the last block's idle groups follow its last sequence and write nothing
+    const int length = length_of(q, b);
+    int n = length;
+    for (int k = lane; k < q.K; k += G)   // past its length too: the loads do not wait for the length
+        if (!passes<T>(q, b, k)) { n = min(n, k); break; }
+#pragma unroll
+    for (int k = G / 2; k; k /= 2) n = min(n, __shfl_xor(n, k));
+    Left<T> left(q, b, n, length);
+    int token = -1;
+    const double u = q.u_sample[b];
+    T p[E], d[E];
+#pragma unroll
+    for (int i = 0; i < E; i++) {
+        const int j = lane * E + i;
+        p[i] = j < q.V ? left.p[j] : T(0.0f);
+        d[i] = left.d && j < q.V ? left.d[j] : T(0.0f);
+    }
+    for (int again = 0; again < 2; again++) {
+        double c[E], own = 0;
+        bool some = false;
+#pragma unroll
+        for (int i = 0; i < E; i++) {
+            const double v = left.of(p[i], d[i], lane * E + i);
+            own += v;
+            c[i] = v > 0 ? own : -1.0;   // the running sum where an action can be drawn
+            some |= v > 0;
+        }
+        const double to = running_sum<G>(own, lane);
+        double before = __shfl_up(to, 1, G);
+        if (lane == 0) before = 0;
+        const double goal = u * __shfl(to, G - 1, G);
+        int pick = -1, last = -1;
+#pragma unroll
+        for (int i = E - 1; i >= 0; i--) {
+            if (c[i] >= 0 && before + c[i] > goal) pick = lane * E + i;
+            if (c[i] >= 0 && last < 0) last = lane * E + i;
+        }
+        const int lo = lowest_lane<G>(pick >= 0), hi = highest_lane<G>(some);
+        const int picked = __shfl(pick, lo % G, G), end = __shfl(last, hi < 0 ? 0 : hi, G);
+        const int found = lo < G ? picked : hi >= 0 ? end : -1;   // rounding can put the goal behind the last element
+        if (token < 0) token = found;
+        const bool retry = token < 0 && !left.whole();   // p nowhere above q: the target's own row
+        if (!__any(retry)) break;
+        if (retry) left.d = nullptr, left.only = -1;
+    }
+    if (!live) return;
+    for (int k = lane; k <= q.K; k += G) put_token(q, b, n, k, token);
+    if (lane == 0) q.accepted[b] = n;
+}
+
+// Wide action sets: one block per sequence.  The row is cut into stretches of four wide loads of a wave; a wave sums whole
+// stretches, the first wave finds the stretch in which the running sum passes the goal and walks that one again.
+template <typename T> constexpr int STRETCH = 4 * 64 * (16 / (int)sizeof(T));
+
+template <typename T> __device__ __forceinline__ void load_stretch(const Left<T> &left, int j0, int V, double (&v)[4][16 / sizeof(T)])
+{
+    constexpr int E = 16 / sizeof(T);
+    const int lane = threadIdx.x % 64;
+    Loose<T, E> p[4], d[4];
+    if (j0 + STRETCH<T> <= V) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const int j = j0 + (i * 64 + lane) * E;
+            p[i] = *(const Loose<T, E> *)(left.p + j);
+            if (left.d) d[i] = *(const Loose<T, E> *)(left.d + j);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+#pragma unroll
+            for (int e = 0; e < E; e++) {
+                const int j = j0 + (i * 64 + lane) * E + e;
+                p[i].v[e] = j < V ? left.p[j] : T(0.0f);
+                d[i].v[e] = left.d && j < V ? left.d[j] : T(0.0f);
+            }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+#pragma unroll
+        for (int e = 0; e < E; e++) v[i][e] = left.of(p[i].v[e], left.d ? d[i].v[e] : T(0.0f), j0 + (i * 64 + lane) * E + e);
+}
+
 template <typename T> __global__ __launch_bounds__(1024) void k_verify(VerifyArgs q)
 {
-    __shared__ int first;
-    __shared__ double red[16], part[16];
-    __shared__ int found;
+    constexpr int E = 16 / sizeof(T);
+    extern __shared__ double part[];   // [stretches]
+    __shared__ int first, found;
     const int b = blockIdx.x, tid = threadIdx.x, lane = tid % 64, w = tid / 64, nw = blockDim.x / 64;
-    int length = q.lengths ? q.lengths[b] : q.K;
-    length = length < 0 ? 0 : length > q.K ? q.K : length;
-    const int n = kept<T>(q, b, length, &first);
-    Left<T> left{(const T *)q.target + (long long)b * q.target_b + (long long)n * q.target_k, nullptr, -1};
-    if (n < length) {
-        if (q.draft) left.d = (const T *)q.draft + (long long)b * q.draft_b + (long long)n * q.draft_k;
-        else left.only = (int)drafted(q, (long long)b * q.K + n);
-    }
+    const int length = length_of(q, b), stretches = (q.V + STRETCH<T> - 1) / STRETCH<T>;
+    if (tid == 0) first = q.K;
+    __syncthreads();
+    for (int k = tid; k < q.K; k += blockDim.x)   // past its length too: the loads do not wait for the length
+        if (!passes<T>(q, b, k)) atomicMin(&first, k);
+    __syncthreads();
+    const int n = min(first, length);
+    Left<T> left(q, b, n, length);
     int token = -1;
-    for (int again = 0; again < 2; again++) {
-        // the range that holds the answer shrinks to the part of one wave until a wave covers it by one element a lane
-        int lo = 0, hi = q.V;
-        double below = 0, goal = 0;
-        bool any = true;
-        while (true) {
-            const int step = (hi - lo + nw - 1) / nw;
-            const int a = min(lo + w * step, hi), z = min(a + step, hi);
-            double s = 0;
-            for (int j = a + lane; j < z; j += 64) s += left.at(j);
+    while (true) {
+        for (int i = w; i < stretches; i += nw) {
+            double v[4][E], s = 0;
+            load_stretch(left, i * STRETCH<T>, q.V, v);
+#pragma unroll
+            for (int a = 0; a < 4; a++)
+#pragma unroll
+                for (int e = 0; e < E; e++) s += v[a][e];
+#pragma unroll
             for (int k = 32; k; k /= 2) s += __shfl_xor(s, k);
-            __syncthreads();
-            if (lane == 0) part[w] = s;
-            __syncthreads();
-            if (lo == 0 && hi == q.V) {
-                double all = 0;
-                for (int i = 0; i < nw; i++) all += part[i];
-                any = all > 0;
-                goal = q.u_sample[b] * all;
-            }
-            if (!any) break;
+            if (lane == 0) part[i] = s;
+        }
+        __syncthreads();
+        if (w == 0) {
+            const int run = (stretches + 63) / 64;
+            double own = 0;
+            for (int i = lane * run; i < min(lane * run + run, stretches); i++) own += part[i];
+            const double to = running_sum<64>(own, lane), goal = q.u_sample[b] * __shfl(to, 63);
             int pick = -1, last = -1;
-            double at = below, last_at = below;
-            for (int i = 0; i < nw; i++) {
-                if (part[i] > 0) last = i, last_at = at;
-                if (part[i] > 0 && at + part[i] > goal) { pick = i; break; }
+            double at = __shfl_up(to, 1), pick_at = 0, last_at = 0;
+            if (lane == 0) at = 0;
+            for (int i = lane * run; i < min(lane * run + run, stretches); i++) {
+                if (part[i] > 0) {
+                    if (pick < 0 && at + part[i] > goal) pick = i, pick_at = at;
+                    last = i, last_at = at;
+                }
                 at += part[i];
             }
-            if (pick < 0) pick = last, at = last_at;   // rounding put the goal behind the last element
-            below = at;
-            const int na = min(lo + pick * step, hi), nz = min(na + step, hi);
-            lo = na, hi = nz;
-            if (hi - lo <= 64) break;
-        }
-        if (any) {
-            if (w == 0) {
-                const double v = lo + lane < hi ? left.at(lo + lane) : 0.0;
-                double c = v;
-                for (int k = 1; k < 64; k *= 2) {
-                    const double o = __shfl_up(c, k);
-                    if (lane >= k) c += o;
+            const int lo = lowest_lane<64>(pick >= 0), hi = highest_lane<64>(last >= 0);
+            int ans = -1;
+            if (hi >= 0) {   // the row has mass
+                const int s = lo < 64 ? __shfl(pick, lo) : __shfl(last, hi);
+                double below = lo < 64 ? __shfl(pick_at, lo) : __shfl(last_at, hi);
+                double v[4][E];
+                load_stretch(left, s * STRETCH<T>, q.V, v);
+                int end = -1;
+#pragma unroll
+                for (int a = 0; a < 4; a++) {
+                    double mine = 0, c[E];
+#pragma unroll
+                    for (int e = 0; e < E; e++) mine += v[a][e], c[e] = mine;
+                    const double incl = running_sum<64>(mine, lane);
+                    double before = __shfl_up(incl, 1);
+                    if (lane == 0) before = 0;
+                    int hit = -1, some = -1;
+#pragma unroll
+                    for (int e = E - 1; e >= 0; e--) {
+                        if (v[a][e] > 0 && below + (before + c[e]) > goal) hit = e;
+                        if (v[a][e] > 0 && some < 0) some = e;
+                    }
+                    const int l = lowest_lane<64>(hit >= 0), h = highest_lane<64>(some >= 0);
+                    const int base = s * STRETCH<T> + a * 64 * E;
+                    const int at_hit = base + (l % 64) * E + __shfl(hit, l % 64), at_end = base + max(h, 0) * E + __shfl(some, max(h, 0));
+                    if (ans < 0 && l < 64) ans = at_hit;
+                    if (h >= 0) end = at_end;
+                    below += __shfl(incl, 63);
                 }
-                const unsigned long long over = __ballot(v > 0 && below + c > goal), some = __ballot(v > 0);
-                if (lane == 0) found = lo + (over ? __ffsll((long long)over) - 1 : 63 - __clzll((long long)some));
+                if (ans < 0) ans = end;   // rounding put the goal behind the last element
             }
-            __syncthreads();
-            token = found;
-            break;
+            if (lane == 0) found = ans;
         }
-        if (!left.d && left.only < 0) break;   // the target itself has nothing: no token
-        left.d = nullptr, left.only = -1;      // p nowhere above q: the target's own row
+        __syncthreads();
+        token = found;
+        if (token >= 0 || left.whole()) break;
+        left.d = nullptr, left.only = -1;   // p nowhere above q: the target's own row
+        __syncthreads();
     }
-    for (int k = tid; k <= q.K; k += blockDim.x) {
-        const long long x = k < n ? drafted(q, (long long)b * q.K + k) : k == n ? token : -1;
-        if (q.token64) ((long long *)q.out)[(long long)b * (q.K + 1) + k] = x;
-        else ((int *)q.out)[(long long)b * (q.K + 1) + k] = (int)x;
-    }
+    for (int k = tid; k <= q.K; k += blockDim.x) put_token(q, b, n, k, token);
     if (tid == 0) q.accepted[b] = n;
 }
 
