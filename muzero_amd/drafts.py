@@ -63,5 +63,5 @@ def verify_drafts(tokens: torch.Tensor, draft: Optional[torch.Tensor], target: t
     args = _engine.PACK_VERIFY(_engine.ELEMENT_TYPES[target.dtype], int(tokens.dtype == torch.int64), B, K, V, 0, p(tokens), p(draft),
                                *sd, p(target), target.stride(0), target.stride(1), p(u_accept), p(u_sample), p(lengths),
                                p(accepted), p(out))
-    _engine.launch_on(target.device, _engine.lib().mz_verify_drafts, args, 'mz_verify_drafts')
+    _engine.call_operator('mz_verify_drafts', target.get_device(), args)
     return accepted, out

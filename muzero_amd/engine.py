@@ -235,14 +235,22 @@ def _stream():
     return C.c_void_p(torch.cuda.current_stream().cuda_stream)
 
 
-def launch_on(device, fn, args: bytes, what):
-    """Calls a tensor operator's entry point with a packed argument struct, on the current stream of `device`, which need not
-    be the current one."""
-    if device.index == torch.cuda.current_device():
-        _check(fn(args, _stream()), what)
+_calls = {}
+
+
+def call_operator(what: str, device: int, args: bytes) -> None:
+    """Calls a tensor operator's entry point with a packed argument struct, on the current stream of the tensors' device (an
+    index, which need not be the current one)."""
+    fn = _calls.get(what)
+    if fn is None:
+        fn = _calls[what] = getattr(lib(), what)
+    if device == torch._C._cuda_getDevice():
+        rc = fn(args, torch._C._cuda_getCurrentRawStream(device))
     else:
         with torch.cuda.device(device):
-            _check(fn(args, _stream()), what)
+            rc = fn(args, torch._C._cuda_getCurrentRawStream(device))
+    if rc:
+        _check(rc, what)
 
 
 class SearchEngine:

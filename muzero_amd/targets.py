@@ -114,37 +114,32 @@ def _like(x: torch.Tensor, channels: bool) -> torch.Tensor:
     return torch.empty(x.shape, dtype=x.dtype, device=x.device) if channels and y.stride(2) != 1 else y
 
 
-def _recurrence_call(backward, gate, x, state, reverse, out, last=None, y=None, out_gate=None, grad_last=None, out_state=None):
-    views = [gate, x, out, y, out_gate]
+def _view(t):
+    return (0, 0, 0, 0) if t is None else (t.data_ptr(), *t.stride())
+
+
+def _at(t):
+    return 0 if t is None else t.data_ptr()
+
+
+def _recurrence_call(what, gate, x, state, reverse, out, last=None, y=None, out_gate=None, grad_last=None, out_state=None):
     B, T, D = x.shape
     if D == 1 and T > 1 and x.stride(1) != 1 and x.stride(0) == 1:
         # one channel, time-major: the rows are the channels of a single sequence
-        views = [None if v is None else v.transpose(0, 2) for v in views]
-        if any(v is not None and v.stride(2) != 1 for v in views):
-            views = [gate, x, out, y, out_gate]
-        else:
+        turned = [None if v is None else v.transpose(0, 2) for v in (gate, x, out, y, out_gate)]
+        if all(v is None or v.stride(2) == 1 for v in turned):
+            gate, x, out, y, out_gate = turned
             B, D = 1, B
-    fields = []
-    for v in views:
-        if v is None:
-            fields += (0, 0, 0, 0)
-        else:
-            fields += (v.data_ptr(), *v.stride())
-    for v in (state, last, grad_last, out_state):
-        fields.append(0 if v is None else v.data_ptr())
-    head = (_engine.ELEMENT_TYPES[x.dtype], B, D, int(reverse), T)
-    L = lib()
-    need = 0
+    args = (_engine.ELEMENT_TYPES[x.dtype], B, D, reverse, T, *_view(gate), *_view(x), *_view(out), *_view(y), *_view(out_gate),
+            _at(state), _at(last), _at(grad_last), _at(out_state))
+    space, need = None, 0
     if T > 256:   # shorter records are never cut into segments
         size = C.c_int64()
-        _check(L.mz_linear_recurrence_workspace(_engine.PACK_RECURRENCE(*head, *fields, 0, 0), int(backward), C.byref(size)))
+        _check(lib().mz_linear_recurrence_workspace(_engine.PACK_RECURRENCE(*args, 0, 0), int(y is not None or grad_last is not None),
+                                                    C.byref(size)))
         need = size.value
-    space = torch.empty(need, dtype=torch.uint8, device=x.device) if need else None
-    args = _engine.PACK_RECURRENCE(*head, *fields, space.data_ptr() if need else 0, need)
-    if backward:
-        _engine.launch_on(x.device, L.mz_linear_recurrence_backward, args, 'mz_linear_recurrence_backward')
-    else:
-        _engine.launch_on(x.device, L.mz_linear_recurrence, args, 'mz_linear_recurrence')
+        space = torch.empty(need, dtype=torch.uint8, device=x.device) if need else None
+    _engine.call_operator(what, x.get_device(), _engine.PACK_RECURRENCE(*args, _at(space), need))
 
 
 def _recurrence_forward(gate, x, state, reverse):
@@ -157,7 +152,7 @@ def _recurrence_forward(gate, x, state, reverse):
     gate, x = _lined_up(gate, channels), _lined_up(x, channels)
     y = _like(x, channels)
     last = torch.empty((B, D), dtype=wide, device=x.device)
-    _recurrence_call(False, gate, x, state, reverse, y, last)
+    _recurrence_call('mz_linear_recurrence', gate, x, state, reverse, y, last)
     return y, last
 
 
@@ -195,8 +190,8 @@ class _LinearRecurrence(torch.autograd.Function):
         dgate = None
         if want_gate:
             y, dgate = _lined_up(y, channels), _like(dy, channels)
-        _recurrence_call(True, gate, dy, state, ctx.reverse, dx, y=y if want_gate else None, out_gate=dgate, grad_last=dlast,
-                         out_state=dstate)
+        _recurrence_call('mz_linear_recurrence_backward', gate, dy, state, ctx.reverse, dx, y=y if want_gate else None,
+                         out_gate=dgate, grad_last=dlast, out_state=dstate)
         return dgate, dx if want_x else None, dstate, None
 
 

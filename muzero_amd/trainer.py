@@ -85,12 +85,14 @@ class _Call:
 
     def run(self, what, grad_loss=None, loss=None, grad=None, stats=None):
         logits, index, teacher, lse, weight = self.kept
-        types = _engine.ELEMENT_TYPES
-        args = _engine.PACK_DISTILL(types[logits.dtype], types[teacher.dtype], int(index.dtype == torch.int64), *logits.shape,
-                                    index.shape[1], self.temperature, logits.data_ptr(), logits.stride(0),
-                                    *[0 if t is None else t.data_ptr() for t in (index, teacher, lse, weight, grad_loss, loss, grad, stats)])
-        if logits.shape[0]:
-            _engine.launch_on(logits.device, getattr(_engine.lib(), what), args, what)
+        at = lambda t: 0 if t is None else t.data_ptr()  # noqa: E731
+        R, V = logits.shape
+        if R:
+            types = _engine.ELEMENT_TYPES
+            _engine.call_operator(what, logits.get_device(), _engine.PACK_DISTILL(
+                types[logits.dtype], types[teacher.dtype], index.dtype == torch.int64, R, V, index.shape[1], self.temperature,
+                logits.data_ptr(), logits.stride(0), index.data_ptr(), teacher.data_ptr(), at(lse), at(weight), at(grad_loss), at(loss),
+                at(grad), at(stats)))
 
 
 class _Distillation(torch.autograd.Function):
