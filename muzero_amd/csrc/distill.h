@@ -228,6 +228,12 @@ struct alignas(16) Raw {
         __builtin_memcpy(&v, w, 16);
         return v;
     }
+    // ... held as four plain registers: the compiler is kept from carrying unpacked values from one step to the next
+    template <typename P> __device__ __forceinline__ P again()
+    {
+        asm("" : "+v"(w[0]), "+v"(w[1]), "+v"(w[2]), "+v"(w[3]));
+        return as<P>();
+    }
     __device__ __forceinline__ void fill(unsigned u) { w[0] = w[1] = w[2] = w[3] = u; }
 };
 template <typename T> __device__ __forceinline__ unsigned lowest_bits();   // a register of -inf
@@ -236,13 +242,13 @@ template <> __device__ __forceinline__ unsigned lowest_bits<__bf16>() { return 0
 template <> __device__ __forceinline__ unsigned lowest_bits<_Float16>() { return 0xfc00fc00u; }
 
 // Wide action sets: one block per row.  A row is a run of whole packs, aligned in memory, between two edges of less than a
-// pack, which the block's last two threads take element by element.  The sums take one pass over the row, four packs of a
-// thread on their way at a time, with a running maximum per thread; the gradient takes another, which in the loss and
-// gradient pass finds the row in cache.
-template <typename T, int THREADS, int MODE>
-__global__ __launch_bounds__(THREADS) void k_distill_row(DistillArgs q, float c)
+// pack, which the block's last two threads take element by element.  The sums take one pass over the row with a running
+// maximum per thread, the gradient another; the loss and gradient pass keeps rows of up to NP packs a thread in registers
+// between the two (NP > 0) and reads wider ones again.
+template <typename T, int THREADS, int NP, int MODE>
+__global__ __launch_bounds__(THREADS, NP ? 6 : 1) void k_distill_row(DistillArgs q, float c)
 {
-    constexpr int E = 16 / sizeof(T), NW = THREADS / 64, U = 2;
+    constexpr int E = 16 / sizeof(T), NW = THREADS / 64, U = NP ? NP : 2;   // packs of a thread on their way at a time
     using P = Pack<T, E>;
     extern __shared__ double lds[];
     __shared__ double red[2][NW];
@@ -414,6 +420,11 @@ __global__ __launch_bounds__(THREADS) void k_distill_row(DistillArgs q, float c)
         };
         if (inner)
             for (int i = start;;) {
+                if constexpr (NP > 0) {
+#pragma unroll
+                    for (int u = 0; u < U; u++) take(i + u * THREADS, r[u].template again<P>());
+                    break;
+                }
                 const int next = i + U * THREADS;
                 Raw ahead[U];
                 if (next < last)
@@ -476,11 +487,11 @@ __global__ __launch_bounds__(THREADS) void k_distill_row(DistillArgs q, float c)
     };
     if (inner)
         for (int i = start; i < last; i += U * THREADS) {
-            if (MODE == 1 || i != start)
+            if (NP == 0 && (MODE == 1 || i != start))
 #pragma unroll
                 for (int u = 0; u < U; u++) r[u] = load(i + u * THREADS);
 #pragma unroll
-            for (int u = 0; u < U; u++) if (i + u * THREADS < last) store(i + u * THREADS, emit(r[u].template as<P>()));
+            for (int u = 0; u < U; u++) if (i + u * THREADS < last) store(i + u * THREADS, emit(r[u].template again<P>()));
         }
     if (edge >= 0) store_edge(emit(load_edge()));
     __syncthreads();

@@ -180,11 +180,10 @@ template <typename T, int G, int E, int MODE> static void launch_group(const Dis
     hipLaunchKernelGGL((k_distill_group<T, G, E, MODE>), dim3((unsigned)(((long long)q.R + rows - 1) / rows)), dim3(256), 0, st, q, c);
 }
 
-constexpr int P64 = 512, P128 = 1024, P256 = 2048, P512 = 8192;
-template <typename T, int THREADS, int MODE> static void launch_row(const DistillArgs &q, float c, hipStream_t st)
+template <typename T, int THREADS, int NP, int MODE> static void launch_row(const DistillArgs &q, float c, hipStream_t st)
 {
     const size_t lds = (size_t)q.K * (8 + 4 + 4) + (q.lse && MODE != 2 ? 4 * (((size_t)q.V + 8 + 31) / 32) : 0);
-    hipLaunchKernelGGL((k_distill_row<T, THREADS, MODE>), dim3((unsigned)q.R), dim3(THREADS), lds, st, q, c);
+    hipLaunchKernelGGL((k_distill_row<T, THREADS, MODE == 1 ? NP : 0, MODE>), dim3((unsigned)q.R), dim3(THREADS), lds, st, q, c);
 }
 
 template <typename T, int MODE> static void launch_distill(const DistillArgs &q, float c, hipStream_t st)
@@ -195,11 +194,12 @@ template <typename T, int MODE> static void launch_distill(const DistillArgs &q,
     else if (q.V <= 64 && q.K <= 64) launch_group<T, 16, 4, MODE>(q, c, st);
     else if (q.V <= 256 && q.K <= 64) launch_group<T, 64, 4, MODE>(q, c, st);
     else if (q.V <= 1024 && q.K <= 64) launch_group<T, 64, 16, MODE>(q, c, st);
-    else if (packs <= P64) launch_row<T, 64, MODE>(q, c, st);
-    else if (packs <= P128) launch_row<T, 128, MODE>(q, c, st);
-    else if (packs <= P256) launch_row<T, 256, MODE>(q, c, st);
-    else if (packs <= P512) launch_row<T, 512, MODE>(q, c, st);
-    else launch_row<T, 1024, MODE>(q, c, st);
+    else if (packs <= 64 * 8) launch_row<T, 64, 8, MODE>(q, c, st);
+    else if (packs <= 128 * 8) launch_row<T, 128, 8, MODE>(q, c, st);
+    else if (packs <= 256 * 8) launch_row<T, 256, 8, MODE>(q, c, st);
+    else if (packs <= 512 * 8) launch_row<T, 512, 8, MODE>(q, c, st);
+    else if (packs <= 8192) launch_row<T, 512, 0, MODE>(q, c, st);
+    else launch_row<T, 1024, 0, MODE>(q, c, st);
 }
 
 template <int MODE> static int run_distill(const mz_distill *a, void *stream, const char *fn)
