@@ -246,7 +246,7 @@ template <> __device__ __forceinline__ unsigned lowest_bits<_Float16>() { return
 // maximum per thread, the gradient another; the loss and gradient pass keeps rows of up to NP packs a thread in registers
 // between the two (NP > 0) and reads wider ones again.
 template <typename T, int THREADS, int NP, int MODE>
-__global__ __launch_bounds__(THREADS, NP ? 6 : 1) void k_distill_row(DistillArgs q, float c)
+__global__ __launch_bounds__(THREADS, NP == 16 ? 4 : NP ? 6 : 1) void k_distill_row(DistillArgs q, float c)
 {
     constexpr int E = 16 / sizeof(T), NW = THREADS / 64, U = NP ? NP : 2;   // packs of a thread on their way at a time
     using P = Pack<T, E>;
@@ -407,37 +407,47 @@ __global__ __launch_bounds__(THREADS, NP ? 6 : 1) void k_distill_row(DistillArgs
     double dsum, dtail;
     if (MODE != 2) {
         // one pass: whenever the thread's maximum rises, what it has summed so far is scaled down to the new one
-        auto take = [&](int i, const P &v) {
-            const float top = top_of(v);
+        auto rise = [&](float top) {
             if (top > m) {
                 const float down = m == -HUGE_VALF ? 0.0f : expo(m - top, c);
                 sum *= down, tail *= down, m = top;
             }
+        };
+        auto take = [&](int i, const P &v) {
             if (m != -HUGE_VALF) add(i, v);
             else
 #pragma unroll
                 for (int k = 0; k < E; k++) if (v.v[k] != v.v[k]) sum = tail = widen(v.v[k]);   // not a number among nothing but -inf
         };
-        if (inner)
-            for (int i = start;;) {
-                if constexpr (NP > 0) {
+        auto take_all = [&](int i) {
+            float top = top_of(r[0].template again<P>());
 #pragma unroll
-                    for (int u = 0; u < U; u++) take(i + u * THREADS, r[u].template again<P>());
-                    break;
+            for (int u = 1; u < U; u++) top = fmaxf(top, top_of(r[u].template again<P>()));
+            rise(top);
+#pragma unroll
+            for (int u = 0; u < U; u++) take(i + u * THREADS, r[u].template again<P>());
+        };
+        if (inner) {
+            if constexpr (NP > 0) take_all(start);
+            else
+                for (int i = start;;) {
+                    const int next = i + U * THREADS;
+                    Raw ahead[U];
+                    if (next < last)
+#pragma unroll
+                        for (int u = 0; u < U; u++) ahead[u] = load(next + u * THREADS);
+                    take_all(i);
+                    if (next >= last) break;
+                    i = next;
+#pragma unroll
+                    for (int u = 0; u < U; u++) r[u] = ahead[u];
                 }
-                const int next = i + U * THREADS;
-                Raw ahead[U];
-                if (next < last)
-#pragma unroll
-                    for (int u = 0; u < U; u++) ahead[u] = load(next + u * THREADS);
-#pragma unroll
-                for (int u = 0; u < U; u++) take(i + u * THREADS, r[u].template as<P>());
-                if (next >= last) break;
-                i = next;
-#pragma unroll
-                for (int u = 0; u < U; u++) r[u] = ahead[u];
-            }
-        if (edge >= 0) take(edge, load_edge());
+        }
+        if (edge >= 0) {
+            const P cut = load_edge();
+            rise(top_of(cut));
+            take(edge, cut);
+        }
         const float own = m;
         m = group_max<64>(m);
         if (lane == 0) red_m[w] = m;

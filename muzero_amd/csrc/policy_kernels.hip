@@ -197,7 +197,7 @@ template <typename T, int MODE> static void launch_distill(const DistillArgs &q,
     else if (packs <= 64 * 8) launch_row<T, 64, 8, MODE>(q, c, st);
     else if (packs <= 128 * 8) launch_row<T, 128, 8, MODE>(q, c, st);
     else if (packs <= 256 * 8) launch_row<T, 256, 8, MODE>(q, c, st);
-    else if (packs <= 512 * 8) launch_row<T, 512, 8, MODE>(q, c, st);
+    else if (packs <= 512 * 8) launch_row<T, 256, 16, MODE>(q, c, st);
     else if (packs <= 8192) launch_row<T, 512, 0, MODE>(q, c, st);
     else launch_row<T, 1024, 0, MODE>(q, c, st);
 }
