@@ -440,7 +440,7 @@ typedef struct mz_recurrence {
     void *last;
     const void *grad_last;
     void *out_state;
-    void *workspace;           /* device memory of this call alone, or NULL where none is needed */
+    void *workspace;           /* device memory of this call alone, 64-byte aligned, or NULL where none is needed */
     int64_t workspace_bytes;
 } mz_recurrence;
 /* Device bytes a call with these arguments needs as workspace (often 0; backward != 0: of the backward call). */

@@ -17,22 +17,22 @@ static size_t size_of(int type) { return type == MZ_F64 ? 8 : type == MZ_F32 ? 4
 
 // ------------------------------------------------------------------------------------------------ recurrence
 
-// Positions a strand holds in registers; below REC_FEW_TILES channel tiles the axis is cut into segments.
+// Positions a strand of k_recurrence_channels holds in registers; from REC_MANY_TILES tiles on a strand is 64 lanes wide;
+// below REC_FEW_TILES, records of at least REC_LEAST_LINKS links are cut into chains.
 constexpr int REC_LENGTH = 8;
-constexpr long long REC_FEW_TILES = 128, REC_WANT_BLOCKS = 512, REC_MAX_SEGMENTS = 64;
+constexpr long long REC_MANY_TILES = 512, REC_FEW_TILES = 256, REC_LEAST_LINKS = 3;
 
 // How a recurrence is run: chosen by sizes, strides and alignment alone, for the workspace query and the call alike.
 struct RecurrencePlan {
     bool channels, brief;    // channels contiguous; so few positions that a thread walks them all
     int vec, lanes;          // channels a thread holds, lanes of a strand
-    int strands, segments;
-    long long segment;
+    int strands, links;      // of a block; of a tile's chain, or 0: one block walks the tile
 };
 
 // VEC = 2 is a 4-byte access of a 16-bit type
 static RecurrencePlan plan_recurrence(const mz_recurrence *a)
 {
-    RecurrencePlan p{true, false, 1, 32, 1, 1, a->T};
+    RecurrencePlan p{true, false, 1, 32, 1, 0};
     uint64_t low = 0;   // low bits of every address and step along the axis and the sequences
     const int size = (int)size_of(a->type);
     for (const mz_strided *t : {&a->gate, &a->x, &a->out, &a->y, &a->out_gate}) {
@@ -52,32 +52,37 @@ static RecurrencePlan plan_recurrence(const mz_recurrence *a)
     }
     p.vec = size == 2 && fits(2) ? 2 : 1;
     auto tiles_of = [&](int lanes) { return (long long)a->B * ((a->D + lanes * p.vec - 1) / (lanes * p.vec)); };
-    p.lanes = tiles_of(64) >= REC_WANT_BLOCKS || tiles_of(32) < REC_FEW_TILES ? 64 : 32;
-    const long long tiles = tiles_of(p.lanes);
-    const int most = REC_THREADS / p.lanes;
-    p.strands = (int)std::min<long long>(most, std::max<long long>(2, (a->T + REC_LENGTH - 1) / REC_LENGTH));
-    if (tiles < REC_FEW_TILES) {
-        const long long rounds = (a->T + (long long)most * REC_LENGTH - 1) / (most * REC_LENGTH);
-        const long long want = std::min<long long>({rounds / 2, (REC_WANT_BLOCKS + tiles - 1) / tiles, REC_MAX_SEGMENTS});
-        if (want > 1) {
-            p.segment = (rounds + want - 1) / want * most * REC_LENGTH;
-            p.segments = (int)((a->T + p.segment - 1) / p.segment);
-        }
-    }
+    p.lanes = tiles_of(64) >= REC_MANY_TILES ? 64 : 32;
+    p.strands = (int)std::min<long long>(REC_THREADS / p.lanes, std::max<long long>(2, (a->T + REC_LENGTH - 1) / REC_LENGTH));
+    const long long links = (a->T + CHAIN_ROWS(size) - 1) / CHAIN_ROWS(size);
+    if (tiles_of(32) < REC_FEW_TILES && links >= REC_LEAST_LINKS && links * tiles_of(64) < INT32_MAX) p.links = (int)links;
     return p;
 }
 
 template <typename T, int VEC, int LANES, bool BWD> static void launch_channels(const RecurrencePlan &p, const RecurrenceArgs &q, hipStream_t st)
 {
     const unsigned tiles = (unsigned)((long long)q.B * ((q.D + LANES * VEC - 1) / (LANES * VEC)));
-    if (q.segments > 1)
-        hipLaunchKernelGGL((k_recurrence_maps<T, VEC, LANES, REC_LENGTH, BWD>), dim3(tiles, q.segments - 1), dim3(REC_THREADS), 0, st, q);
-    hipLaunchKernelGGL((k_recurrence_channels<T, VEC, LANES, REC_LENGTH, BWD>), dim3(tiles, q.segments), dim3(LANES * p.strands), 0, st, q);
+    hipLaunchKernelGGL((k_recurrence_channels<T, VEC, LANES, REC_LENGTH, BWD>), dim3(tiles), dim3(LANES * p.strands), 0, st, q);
+}
+
+static size_t granule_count(const mz_recurrence *a, const RecurrencePlan &p)
+{
+    return p.links ? 8 + (size_t)p.links * a->B * a->D * 3 * (a->type == MZ_F64 ? 2 : 1) : 0;
+}
+
+template <typename T, int VEC, bool BWD> static void launch_chain(const RecurrenceArgs &q, hipStream_t st)
+{
+    const long long granules = 8 + (long long)q.links * q.B * q.D * 3 * (long long)(sizeof(acc_t<T>) / 4);
+    const unsigned blocks = (unsigned)std::min<long long>((granules + 255) / 256, 2048);
+    hipLaunchKernelGGL(k_zero_granules, dim3(blocks), dim3(256), 0, st, q.granules, granules);
+    const long long tiles = (long long)q.B * ((q.D + 64 * VEC - 1) / (64 * VEC));
+    hipLaunchKernelGGL((k_recurrence_chain<T, VEC, BWD>), dim3((unsigned)(tiles * q.links)), dim3(64 * CHAIN_WAVES), 0, st, q);
 }
 
 template <typename T, int VEC, bool BWD> static void launch_channels(const RecurrencePlan &p, const RecurrenceArgs &q, hipStream_t st)
 {
-    if (p.lanes == 64) launch_channels<T, VEC, 64, BWD>(p, q, st);
+    if (p.links) launch_chain<T, VEC, BWD>(q, st);
+    else if (p.lanes == 64) launch_channels<T, VEC, 64, BWD>(p, q, st);
     else launch_channels<T, VEC, 32, BWD>(p, q, st);
 }
 
@@ -108,11 +113,6 @@ template <typename T, bool BWD> static void launch_recurrence(const RecurrencePl
     else launch_channels<T, 1, BWD>(p, q, st);
 }
 
-static size_t maps_bytes(const mz_recurrence *a, const RecurrencePlan &p)
-{
-    return (size_t)(p.segments - 1) * 2 * a->B * a->D * (a->type == MZ_F64 ? 8 : 4);
-}
-
 static int check_recurrence(const mz_recurrence *a, bool backward, const char *fn)
 {
     if (!a) return api_fail(MZ_ERR_ARG, std::string(fn) + ": null argument");
@@ -130,10 +130,10 @@ template <bool BWD> static int run_recurrence(const mz_recurrence *a, void *stre
     (void)hipGetLastError();
     if (int rc = check_recurrence(a, BWD, fn)) return rc;
     const RecurrencePlan p = plan_recurrence(a);
-    if (a->workspace_bytes < (int64_t)maps_bytes(a, p) || (p.segments > 1 && !a->workspace))
-        return api_fail(MZ_ERR_ARG, std::string(fn) + ": the workspace is smaller than mz_linear_recurrence_workspace says");
+    if (p.links && (a->workspace_bytes < (int64_t)(8 * granule_count(a, p)) || !a->workspace || (uintptr_t)a->workspace % 64))
+        return api_fail(MZ_ERR_ARG, std::string(fn) + ": the workspace is smaller than mz_linear_recurrence_workspace says, or not aligned to 64 bytes");
     RecurrenceArgs q{};
-    q.B = a->B, q.D = a->D, q.T = a->T, q.maps = a->workspace, q.segments = p.segments, q.segment = p.segment;
+    q.B = a->B, q.D = a->D, q.T = a->T, q.granules = (unsigned long long *)a->workspace, q.links = p.links;
     // the pass runs along the axis, or against it: reversed recurrence and gradient each turn it round
     const bool turned = (a->reverse != 0) != BWD;
     auto view = [&](const mz_strided &t) {
@@ -168,7 +168,7 @@ extern "C" int mz_linear_recurrence_workspace(const mz_recurrence *args_h, int32
 {
     if (int rc = check_recurrence(args_h, backward != 0, "mz_linear_recurrence_workspace")) return rc;
     if (!out_bytes) return api_fail(MZ_ERR_ARG, "mz_linear_recurrence_workspace: null argument");
-    *out_bytes = (int64_t)maps_bytes(args_h, plan_recurrence(args_h));
+    *out_bytes = (int64_t)(8 * granule_count(args_h, plan_recurrence(args_h)));
     return MZ_OK;
 }
 

@@ -25,9 +25,8 @@ struct RecurrenceArgs {
     const void *first;   // acc[B][D] what goes into position 0 (backward: gradient of the last state), NULL = 0
     const void *state0;  // backward: acc[B][D] the forward pass's first state, NULL = 0
     void *last;          // acc[B][D] the state behind the last position (backward: gradient of the first state), may be NULL
-    void *maps;          // acc[segments - 1][2][B][D] maps of all segments but the last, or NULL: one segment
-    int segments;
-    long long segment;   // positions per segment
+    unsigned long long *granules;   // k_recurrence_chain: a counter of 64 bytes, then what its links hand on, zero before the call
+    int links;
 };
 
 template <typename T> __device__ __forceinline__ const T *at(const RecurrenceArgs::View &v, int b, long long s, int d)
@@ -68,6 +67,34 @@ template <typename T, int VEC, int L, bool BWD> struct Strand {
 #pragma unroll
                     for (int j = 0; j < VEC; j++) a[i].v[j] = T(1.0f), x[i].v[j] = T(0.0f);
     }
+    // The strand's outputs from the state h in front of it.
+    __device__ __forceinline__ void walk(const RecurrenceArgs &q, int b, long long s0, long long end, int d, bool want_da, acc_t<T> (&h)[VEC]) const
+    {
+        using A = acc_t<T>;
+        const int left = (int)min((long long)L, max(end - s0, 0ll));
+#pragma unroll
+        for (int i = 0; i < L; i++) {
+            if (i >= left) continue;
+            P o, da;
+#pragma unroll
+            for (int j = 0; j < VEC; j++) {
+                h[j] = fma_acc(widen(a[i].v[j]), h[j], widen(x[i].v[j]));
+                o.v[j] = narrow<T>(h[j]);
+            }
+            *(P *)at<T>(q.out, b, s0 + i, d) = o;
+            if constexpr (BWD) {
+                if (want_da) {
+                    const bool first = s0 + i + 1 == q.T;   // of the forward pass: what precedes it is the first state
+#pragma unroll
+                    for (int j = 0; j < VEC; j++) {
+                        const A before = first ? state_at<A>(q.state0, (long long)b * q.D + d + j) : widen(y[i].v[j]);
+                        da.v[j] = narrow<T>(h[j] * before);
+                    }
+                    *(P *)at<T>(q.da, b, s0 + i, d) = da;
+                }
+            }
+        }
+    }
     // The strand's map behind the map (ra, rx).
     __device__ __forceinline__ void compose(acc_t<T> (&ra)[VEC], acc_t<T> (&rx)[VEC]) const
     {
@@ -93,8 +120,6 @@ constexpr int REC_THREADS = 512;   // of a block: strands of 32 or 64 lanes alon
 // Channels contiguous: LANES neighbouring lanes hold LANES * VEC neighbouring channels (a "strand") and walk L consecutive
 // positions in registers; the block's strands follow each other in time and exchange their maps through LDS,
 // one barrier per round of strands, while the next round's loads are on their way.
-// A grid of few channel tiles leaves compute units idle: the axis is then cut into segments of one block each, whose maps
-// k_recurrence_maps has left in memory; a block folds those of the segments before its own.
 template <typename T, int VEC, int LANES, int L, bool BWD>
 __global__ __launch_bounds__(REC_THREADS) void k_recurrence_channels(RecurrenceArgs q)
 {
@@ -105,36 +130,27 @@ __global__ __launch_bounds__(REC_THREADS) void k_recurrence_channels(RecurrenceA
     __shared__ Map run[2][STRANDS][LANES];
     const int nv = blockDim.x / LANES;
     const int tiles = (q.D + LANES * VEC - 1) / (LANES * VEC);
-    // segments of one tile run from the last to the first: what the maps' pass read last is read first
-    const int seg = q.segments - 1 - blockIdx.y;
     const int tile = tile_index();
     const int b = tile / tiles, c = threadIdx.x % LANES, v = threadIdx.x / LANES;
     const int d0 = (tile % tiles) * LANES * VEC + c * VEC;
     const bool live = d0 < q.D;
     const int d = live ? d0 : q.D - VEC;   // idle lanes read what the last live one reads
     const long long row = (long long)b * q.D + d;
-    const long long begin = seg * q.segment, end = min(begin + q.segment, q.T);
+    const long long end = q.T;
     const bool want_da = BWD && q.da.p;
     A carry[VEC];
 #pragma unroll
     for (int j = 0; j < VEC; j++) carry[j] = state_at<A>(q.first, row + j);
-    const long long rows = (long long)q.B * q.D;
-#pragma unroll 4
-    for (int i = 0; i < seg; i++) {
-        const A *m = (const A *)q.maps + (long long)i * 2 * rows + row;
-#pragma unroll
-        for (int j = 0; j < VEC; j++) carry[j] = fma_acc(m[j], carry[j], m[rows + j]);
-    }
     const int round = nv * L;
     int buf = 0;
     Strand<T, VEC, L, BWD> now, next;
-    const long long inside = BWD ? min(end, q.T - 1) : end;   // a round that ends here or earlier needs no clamping
+    const long long inside = BWD ? end - 1 : end;   // a round that ends here or earlier needs no clamping
     auto load = [&](Strand<T, VEC, L, BWD> &w, long long base) {
         if (base + round <= inside) w.template load<true>(q, b, base + v * L, end, d, want_da);
         else w.template load<false>(q, b, base + v * L, end, d, want_da);
     };
-    load(now, begin);
-    for (long long base = begin; base < end; base += round, buf ^= 1) {
+    load(now, 0);
+    for (long long base = 0; base < end; base += round, buf ^= 1) {
         const bool more = base + round < end;
         if (more) load(next, base + round);
         Map m;
@@ -153,32 +169,10 @@ __global__ __launch_bounds__(REC_THREADS) void k_recurrence_channels(RecurrenceA
             }
         }
         const long long s0 = base + v * L;
-        const int left = live ? (int)min((long long)L, max(end - s0, 0ll)) : 0;
-#pragma unroll
-        for (int i = 0; i < L; i++) {
-            if (i >= left) break;
-            P o, da;
-#pragma unroll
-            for (int j = 0; j < VEC; j++) {
-                h[j] = fma_acc(widen(now.a[i].v[j]), h[j], widen(now.x[i].v[j]));
-                o.v[j] = narrow<T>(h[j]);
-            }
-            *(P *)at<T>(q.out, b, s0 + i, d) = o;
-            if constexpr (BWD) {
-                if (want_da) {
-                    const bool first = s0 + i + 1 == q.T;   // of the forward pass: what precedes it is the first state
-#pragma unroll
-                    for (int j = 0; j < VEC; j++) {
-                        const A before = first ? state_at<A>(q.state0, row + j) : widen(now.y[i].v[j]);
-                        da.v[j] = narrow<T>(h[j] * before);
-                    }
-                    *(P *)at<T>(q.da, b, s0 + i, d) = da;
-                }
-            }
-        }
+        now.walk(q, b, s0, live ? end : s0, d, want_da, h);
         if (more) now = next;
     }
-    if (q.last && live && v == 0 && seg == q.segments - 1) {
+    if (q.last && live && v == 0) {
 #pragma unroll
         for (int j = 0; j < VEC; j++) {
             A z = carry[j];
@@ -188,53 +182,141 @@ __global__ __launch_bounds__(REC_THREADS) void k_recurrence_channels(RecurrenceA
     }
 }
 
-// The maps of all segments but the last: every strand of a block composes a stretch of its own, and the first strand folds
-// the stretches.
-template <typename T, int VEC, int LANES, int L, bool BWD>
-__global__ __launch_bounds__(REC_THREADS) void k_recurrence_maps(RecurrenceArgs q)
+// Long records of few channels: a block for every tile would leave compute units idle, so the axis is cut into links of
+// 256 positions (128 in float64) and every link of a tile is a block of its own, with its inputs in registers from the first read to
+// the output.  A link hands two things on through memory: its map, as soon as it has it, and the state behind it, once it
+// knows the state in front.  To learn that, it looks back over its predecessors: past those that have only a map yet, to one
+// whose state is known, and folds the maps in between from there on - the same operations in the same order however far it
+// had to look, so results do not depend on timing.
+// A value travels as an 8-byte granule of its 32 bits and a tag, written and read as one access at the scope of the device;
+// granules are zero before the call.  Links are dealt by a counter, so a block waits for blocks only that are already running
+// and that wait for earlier ones in turn: every wait ends.
+constexpr int CHAIN_WAVES = 16, CHAIN_BACK = 16;
+constexpr int CHAIN_LENGTH(int size) { return size == 8 ? 8 : 16; }   // positions of a wave; float64 takes twice the registers
+constexpr int CHAIN_ROWS(int size) { return CHAIN_LENGTH(size) * CHAIN_WAVES; }
+
+template <typename A> __device__ __forceinline__ void granule_put(unsigned long long *to, A v)
 {
-    constexpr int STRANDS = REC_THREADS / LANES;
+    unsigned w[sizeof(A) / 4];
+    __builtin_memcpy(w, &v, sizeof(A));
+#pragma unroll
+    for (int i = 0; i < (int)(sizeof(A) / 4); i++)
+        __hip_atomic_store(to + i, (unsigned long long)w[i] << 32 | 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+template <typename A> __device__ __forceinline__ bool granule_get(const unsigned long long *from, A &v)
+{
+    unsigned w[sizeof(A) / 4];
+    bool there = true;
+#pragma unroll
+    for (int i = 0; i < (int)(sizeof(A) / 4); i++) {
+        const unsigned long long g = __hip_atomic_load(from + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        w[i] = (unsigned)(g >> 32);
+        there &= (unsigned)g == 1u;
+    }
+    __builtin_memcpy(&v, w, sizeof(A));
+    return there;
+}
+
+__global__ void k_zero_granules(unsigned long long *p, long long n)
+{
+    for (long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += (long long)gridDim.x * blockDim.x) p[i] = 0;
+}
+
+template <typename T, int VEC, bool BWD>
+__global__ __launch_bounds__(64 * CHAIN_WAVES) void k_recurrence_chain(RecurrenceArgs q)
+{
     using A = acc_t<T>;
+    using P = Pack<T, VEC>;
+    constexpr int L = CHAIN_LENGTH(sizeof(T)), ROWS = CHAIN_ROWS(sizeof(T)), W = sizeof(A) / 4;
     struct Map { A a[VEC], x[VEC]; };
-    __shared__ Map run[STRANDS][LANES];
-    const int tiles = (q.D + LANES * VEC - 1) / (LANES * VEC);
-    const int seg = blockIdx.y;
-    const int tile = tile_index();
-    const int b = tile / tiles, c = threadIdx.x % LANES, v = threadIdx.x / LANES;
-    const int d0 = (tile % tiles) * LANES * VEC + c * VEC;
+    struct State { A h[VEC]; };
+    __shared__ Map run[CHAIN_WAVES][64], back[CHAIN_BACK][64];
+    __shared__ State front[64];
+    __shared__ unsigned ticket;
+    if (threadIdx.x == 0) ticket = atomicAdd((unsigned *)q.granules, 1u);
+    __syncthreads();
+    const int tiles = (q.D + 64 * VEC - 1) / (64 * VEC), all = tiles * q.B;
+    const int link = (int)(ticket / (unsigned)all), tile = (int)(ticket % (unsigned)all);
+    const int b = tile / tiles, c = threadIdx.x % 64, v = threadIdx.x / 64;
+    const int d0 = (tile % tiles) * 64 * VEC + c * VEC;
     const bool live = d0 < q.D;
     const int d = live ? d0 : q.D - VEC;
-    const long long stretch = ((q.segment + STRANDS - 1) / STRANDS + L - 1) / L * L;
-    const long long last = (seg + 1) * q.segment;   // below T: the last segment's map is not needed
-    const long long begin = min(seg * q.segment + v * stretch, last), end = min(begin + stretch, last);
+    const long long row = (long long)b * q.D + d, s0 = (long long)link * ROWS + v * L;
+    const long long end = min((link + 1ll) * ROWS, q.T);
+    const bool want_da = BWD && q.da.p;
+    Strand<T, VEC, L, BWD> w;
+    if (end + (BWD ? 1 : 0) <= q.T && end == (link + 1ll) * ROWS) w.template load<true>(q, b, s0, end, d, want_da);
+    else w.template load<false>(q, b, s0, end, d, want_da);
     Map m;
 #pragma unroll
     for (int j = 0; j < VEC; j++) m.a[j] = A(1), m.x[j] = A(0);
-    Strand<T, VEC, L, BWD> now, next;
-    auto load = [&](Strand<T, VEC, L, BWD> &w, long long s) {
-        if (s + L <= end) w.template load<true>(q, b, s, end, d, false);
-        else w.template load<false>(q, b, s, end, d, false);
-    };
-    if (begin < end) load(now, begin);
-    for (long long s = begin; s < end; s += L) {
-        const bool more = s + L < end;
-        if (more) load(next, s + L);
-        now.compose(m.a, m.x);
-        if (more) now = next;
-    }
+    w.compose(m.a, m.x);
     run[v][c] = m;
-    __syncthreads();
-    if (v == 0 && live) {
-        for (int i = 1; i < STRANDS; i++) {
+    lds_fence_barrier();
+    if (v == 0) {
+        // granules of a channel and link: map (a, x), then the state behind it
+        auto place = [&](int l, int j) { return q.granules + 8 + (((long long)l * q.B * q.D + row + j) * 3) * W; };
+        for (int i = 1; i < CHAIN_WAVES; i++) {
             const Map o = run[i][c];
 #pragma unroll
             for (int j = 0; j < VEC; j++) m.x[j] = fma_acc(o.a[j], m.x[j], o.x[j]), m.a[j] *= o.a[j];
         }
-        const long long rows = (long long)q.B * q.D;
-        A *to = (A *)q.maps + (long long)seg * 2 * rows + (long long)b * q.D + d;
+        A h[VEC];
+        if (link == 0) {
 #pragma unroll
-        for (int j = 0; j < VEC; j++) to[j] = m.a[j], to[rows + j] = m.x[j];
+            for (int j = 0; j < VEC; j++) h[j] = state_at<A>(q.first, row + j);
+        } else {
+#pragma unroll
+            for (int j = 0; j < VEC; j++) granule_put(place(link, j), m.a[j]), granule_put(place(link, j) + W, m.x[j]);
+            int n = 0;   // maps looked past
+            while (true) {
+                const int l = link - 1 - n;   // >= 0: link 0 hands on its state alone, the look back ends there at the latest
+                bool known = true, mapped = true;
+                Map o;
+#pragma unroll
+                for (int j = 0; j < VEC; j++) {
+                    known &= granule_get(place(l, j) + 2 * W, h[j]);
+                    mapped &= granule_get(place(l, j), o.a[j]);
+                    mapped &= granule_get(place(l, j) + W, o.x[j]);
+                }
+                if (__all(known)) break;
+                if (n < CHAIN_BACK && __all(mapped)) back[n++][c] = o;
+                else __builtin_amdgcn_s_sleep(1);
+            }
+            for (int i = n - 1; i >= 0; i--) {
+                const Map o = back[i][c];
+#pragma unroll
+                for (int j = 0; j < VEC; j++) h[j] = fma_acc(o.a[j], h[j], o.x[j]);
+            }
+        }
+        State behind, before;
+#pragma unroll
+        for (int j = 0; j < VEC; j++) {
+            before.h[j] = h[j];
+            behind.h[j] = fma_acc(m.a[j], h[j], m.x[j]);
+            if (link + 1 < q.links) granule_put(place(link, j) + 2 * W, behind.h[j]);
+        }
+        front[c] = before;
+        if (q.last && live && link + 1 == q.links) {
+#pragma unroll
+            for (int j = 0; j < VEC; j++) {
+                A z = behind.h[j];
+                if (BWD) z *= widen(at<T>(q.a, b, q.T - 1, d)[j]);
+                ((A *)q.last)[row + j] = z;
+            }
+        }
     }
+    lds_fence_barrier();
+    const State before = front[c];
+    A h[VEC];
+#pragma unroll
+    for (int j = 0; j < VEC; j++) h[j] = before.h[j];
+    for (int i = 0; i < v; i++) {
+        const Map o = run[i][c];
+#pragma unroll
+        for (int j = 0; j < VEC; j++) h[j] = fma_acc(o.a[j], h[j], o.x[j]);
+    }
+    w.walk(q, b, s0, live ? end : s0, d, want_da, h);
 }
 
 // Few positions (a step of serving, short records): a thread walks VEC channels of one sequence through all of them.
@@ -256,28 +338,7 @@ __global__ __launch_bounds__(256) void k_recurrence_short(RecurrenceArgs q)
     for (long long s0 = 0; s0 < q.T; s0 += L) {
         Strand<T, VEC, L, BWD> w;
         w.template load<false>(q, b, s0, q.T, d, want_da);
-#pragma unroll
-        for (int i = 0; i < L; i++) {
-            if (s0 + i >= q.T) break;
-            P o, da;
-#pragma unroll
-            for (int j = 0; j < VEC; j++) {
-                h[j] = fma_acc(widen(w.a[i].v[j]), h[j], widen(w.x[i].v[j]));
-                o.v[j] = narrow<T>(h[j]);
-            }
-            *(P *)at<T>(q.out, b, s0 + i, d) = o;
-            if constexpr (BWD) {
-                if (want_da) {
-                    const bool first = s0 + i + 1 == q.T;
-#pragma unroll
-                    for (int j = 0; j < VEC; j++) {
-                        const A before = first ? state_at<A>(q.state0, row + j) : widen(w.y[i].v[j]);
-                        da.v[j] = narrow<T>(h[j] * before);
-                    }
-                    *(P *)at<T>(q.da, b, s0 + i, d) = da;
-                }
-            }
-        }
+        w.walk(q, b, s0, q.T, d, want_da, h);
     }
     if (q.last)
 #pragma unroll

@@ -133,7 +133,7 @@ def _recurrence_call(what, gate, x, state, reverse, out, last=None, y=None, out_
     args = (_engine.ELEMENT_TYPES[x.dtype], B, D, reverse, T, *_view(gate), *_view(x), *_view(out), *_view(y), *_view(out_gate),
             _at(state), _at(last), _at(grad_last), _at(out_state))
     space, need = None, 0
-    if T > 256:   # shorter records are never cut into segments
+    if T > 256:   # shorter records need none
         size = C.c_int64()
         _check(lib().mz_linear_recurrence_workspace(_engine.PACK_RECURRENCE(*args, 0, 0), int(y is not None or grad_last is not None),
                                                     C.byref(size)))
