@@ -7,6 +7,7 @@ from __future__ import annotations
 
 from typing import Optional, Tuple
 
+import numpy as np
 import torch
 
 from . import engine as _engine
@@ -25,13 +26,14 @@ def verify_drafts(tokens: torch.Tensor, draft: Optional[torch.Tensor], target: t
     negative, infinite or NaN count as 0, a drafted move outside 0..V-1 is not kept.
     Returns (accepted int32 [B], moves [B, K + 1] of the type of tokens: the kept drafts, the drawn move, -1 behind it; a
     target row without any mass yields -1)."""
-    named = (('tokens', tokens), ('draft', draft), ('target', target), ('u_accept', u_accept), ('u_sample', u_sample), ('lengths', lengths))
-    for name, t in named:
+    where = target.get_device() if torch.is_tensor(target) else -1
+    for name, t in (('target', target), ('tokens', tokens), ('draft', draft), ('u_accept', u_accept), ('u_sample', u_sample),
+                    ('lengths', lengths)):
         if t is None and name in ('draft', 'lengths'):
             continue
         if not torch.is_tensor(t) or not t.is_cuda:
             raise _engine.EngineError(f'verify_drafts needs device tensors (there is no CPU fallback): {name}')
-        if t.device != target.device:
+        if t.get_device() != where:
             raise ValueError(f'verify_drafts: {name} is on another device than the target')
     if tokens.dim() != 2 or target.dim() != 3:
         raise ValueError('verify_drafts: tokens [B, K] and target [B, K + 1, V] expected')
@@ -48,8 +50,8 @@ def verify_drafts(tokens: torch.Tensor, draft: Optional[torch.Tensor], target: t
         raise ValueError('verify_drafts: u_accept [B, K] and u_sample [B] must be float64')
     if lengths is not None and (tuple(lengths.shape) != (B,) or lengths.dtype != torch.int32):
         raise ValueError('verify_drafts: lengths must be int32 [B]')
-    accepted = torch.empty(B, dtype=torch.int32, device=target.device)
-    out = torch.empty((B, K + 1), dtype=tokens.dtype, device=target.device)
+    accepted = u_sample.new_empty((B,), dtype=torch.int32)
+    out = tokens.new_empty((B, K + 1))
     if B == 0:
         return accepted, out
     if target.stride(2) != 1 and V > 1:
@@ -63,5 +65,31 @@ def verify_drafts(tokens: torch.Tensor, draft: Optional[torch.Tensor], target: t
     args = _engine.PACK_VERIFY(_engine.ELEMENT_TYPES[target.dtype], int(tokens.dtype == torch.int64), B, K, V, 0, p(tokens), p(draft),
                                *sd, p(target), target.stride(0), target.stride(1), p(u_accept), p(u_sample), p(lengths),
                                p(accepted), p(out))
-    _engine.call_operator('mz_verify_drafts', target.get_device(), args)
+    _engine.call_operator('mz_verify_drafts', where, args)
     return accepted, out
+
+
+def verify_by_search(mcts, network, observations, legal_actions, to_play, tokens: torch.Tensor, draft: Optional[torch.Tensor],
+                     temperature: float = 1.0, lengths: Optional[torch.Tensor] = None, action_encoder=None, seed: int = 0,
+                     tree_id0: int = 0) -> Tuple[torch.Tensor, torch.Tensor, np.ndarray]:
+    """Moves drafted K ahead in B games against the search's own policies: one `search_batch` over all B * (K + 1) positions
+    the drafts passed through, then `verify_drafts` with uniforms drawn from `np.random` behind the search's noise (B * K for
+    the drafts, then B for the draws).
+
+    observations [B, K + 1, ...], legal_actions [B, K + 1, A], to_play [B, K + 1]: the position in front of every drafted move
+    and the one behind the last (behind a game's own length: any position).  tokens [B, K] device int32 / int64, draft
+    [B, K, A] device float64 or None.  At `temperature` 0 the searched policy is its best move alone.
+    Returns (accepted, moves, root values [B, K + 1])."""
+    B, K = tokens.shape
+    observations = observations if torch.is_tensor(observations) else np.asarray(observations)
+    n = B * (K + 1)
+    if tuple(observations.shape[:2]) != (B, K + 1):
+        raise ValueError(f'verify_by_search: observations must be [{B}, {K + 1}, ...], got {tuple(observations.shape)}')
+    _, values, probs = mcts.search_batch(network, observations.reshape((n,) + tuple(observations.shape[2:])),
+                                         np.asarray(legal_actions).reshape(n, -1), np.asarray(to_play).reshape(n), temperature,
+                                         action_encoder=action_encoder, seed=seed, tree_id0=tree_id0)
+    on = lambda a: torch.as_tensor(np.ascontiguousarray(a, dtype=np.float64), device=tokens.device)  # noqa: E731
+    target = on(np.stack([np.asarray(p) for p in probs]) if not isinstance(probs, np.ndarray) else probs).reshape(B, K + 1, -1)
+    u_accept, u_sample = np.random.random_sample((B, K)), np.random.random_sample(B)
+    accepted, moves = verify_drafts(tokens, draft, target, on(u_accept), on(u_sample), lengths=lengths)
+    return accepted, moves, np.asarray(values, dtype=np.float64).reshape(B, K + 1)

@@ -151,7 +151,7 @@ def _recurrence_forward(gate, x, state, reverse):
     channels = D > 1 and (x.stride(2) == 1 or x.stride(1) != 1)
     gate, x = _lined_up(gate, channels), _lined_up(x, channels)
     y = _like(x, channels)
-    last = torch.empty((B, D), dtype=wide, device=x.device)
+    last = x.new_empty((B, D), dtype=wide)
     _recurrence_call('mz_linear_recurrence', gate, x, state, reverse, y, last)
     return y, last
 
@@ -207,17 +207,21 @@ def linear_recurrence(gate: torch.Tensor, x: torch.Tensor, state: Optional[torch
     ensures; a gate of 0 cuts the record."""
     if not (torch.is_tensor(gate) and torch.is_tensor(x) and gate.is_cuda and x.is_cuda):
         raise _engine.EngineError('linear_recurrence needs device tensors (there is no CPU fallback)')
-    if x.dim() != 3 or gate.shape != x.shape:
-        raise ValueError(f'linear_recurrence: gate and x must both be [B, T, D], got {tuple(gate.shape)} and {tuple(x.shape)}')
-    if x.dtype not in _engine.ELEMENT_TYPES or gate.dtype != x.dtype:
-        raise ValueError(f'linear_recurrence: gate and x must share a floating type, got {gate.dtype} and {x.dtype}')
-    if gate.device != x.device:
+    shape, dtype = x.shape, x.dtype
+    if len(shape) != 3 or gate.shape != shape:
+        raise ValueError(f'linear_recurrence: gate and x must both be [B, T, D], got {tuple(gate.shape)} and {tuple(shape)}')
+    if dtype not in _engine.ELEMENT_TYPES or gate.dtype != dtype:
+        raise ValueError(f'linear_recurrence: gate and x must share a floating type, got {gate.dtype} and {dtype}')
+    if gate.get_device() != x.get_device():
         raise ValueError('linear_recurrence: gate and x are on different devices')
+    grads = gate.requires_grad or x.requires_grad
     if state is not None:
-        if state.shape != (x.shape[0], x.shape[2]) or state.dtype != _STATE_TYPE.get(x.dtype, torch.float32) or state.device != x.device:
-            raise ValueError(f'linear_recurrence: state must be {_STATE_TYPE.get(x.dtype, torch.float32)} [B, D] on the device of x')
+        wide = _STATE_TYPE.get(dtype, torch.float32)
+        if not torch.is_tensor(state) or state.shape != (shape[0], shape[2]) or state.dtype != wide or state.get_device() != x.get_device():
+            raise ValueError(f'linear_recurrence: state must be {wide} [{shape[0]}, {shape[2]}] on the device of x')
         state = state.contiguous()
-    if torch.is_grad_enabled() and (gate.requires_grad or x.requires_grad or (state is not None and state.requires_grad)):
+        grads = grads or state.requires_grad
+    if grads and torch.is_grad_enabled():
         return _LinearRecurrence.apply(gate, x, state, bool(reverse))
     return _recurrence_forward(gate, x, state, bool(reverse))
 
