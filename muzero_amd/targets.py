@@ -124,14 +124,19 @@ def _at(t):
 
 def _recurrence_call(what, gate, x, state, reverse, out, last=None, y=None, out_gate=None, grad_last=None, out_state=None):
     B, T, D = x.shape
-    if D == 1 and T > 1 and x.stride(1) != 1 and x.stride(0) == 1:
-        # one channel, time-major: the rows are the channels of a single sequence
-        turned = [None if v is None else v.transpose(0, 2) for v in (gate, x, out, y, out_gate)]
-        if all(v is None or v.stride(2) == 1 for v in turned):
-            gate, x, out, y, out_gate = turned
-            B, D = 1, B
-    args = (_engine.ELEMENT_TYPES[x.dtype], B, D, reverse, T, *_view(gate), *_view(x), *_view(out), *_view(y), *_view(out_gate),
-            _at(state), _at(last), _at(grad_last), _at(out_state))
+    if x.is_contiguous() and gate.is_contiguous() and out.is_contiguous() and (y is None or y.is_contiguous() and out_gate.is_contiguous()):
+        n = T * D
+        args = (_engine.ELEMENT_TYPES[x.dtype], B, D, reverse, T, gate.data_ptr(), n, D, 1, x.data_ptr(), n, D, 1,
+                out.data_ptr(), n, D, 1, _at(y), n, D, 1, _at(out_gate), n, D, 1, _at(state), _at(last), _at(grad_last), _at(out_state))
+    else:
+        if D == 1 and T > 1 and x.stride(1) != 1 and x.stride(0) == 1:
+            # one channel, time-major: the rows are the channels of a single sequence
+            turned = [None if v is None else v.transpose(0, 2) for v in (gate, x, out, y, out_gate)]
+            if all(v is None or v.stride(2) == 1 for v in turned):
+                gate, x, out, y, out_gate = turned
+                B, D = 1, B
+        args = (_engine.ELEMENT_TYPES[x.dtype], B, D, reverse, T, *_view(gate), *_view(x), *_view(out), *_view(y), *_view(out_gate),
+                _at(state), _at(last), _at(grad_last), _at(out_state))
     space, need = None, 0
     if T > 256:   # shorter records need none
         size = C.c_int64()
@@ -146,12 +151,10 @@ def _recurrence_forward(gate, x, state, reverse):
     B, T, D = x.shape
     wide = _STATE_TYPE.get(x.dtype, torch.float32)
     if x.numel() == 0:
-        last = torch.zeros((B, D), dtype=wide, device=x.device) if state is None else state.clone()
-        return torch.empty_like(x), last
+        return torch.empty_like(x), torch.zeros((B, D), dtype=wide, device=x.device) if state is None else state.clone()
     channels = D > 1 and (x.stride(2) == 1 or x.stride(1) != 1)
     gate, x = _lined_up(gate, channels), _lined_up(x, channels)
-    y = _like(x, channels)
-    last = x.new_empty((B, D), dtype=wide)
+    y, last = _like(x, channels), x.new_empty((B, D), dtype=wide)
     _recurrence_call('mz_linear_recurrence', gate, x, state, reverse, y, last)
     return y, last
 
@@ -162,36 +165,33 @@ class _LinearRecurrence(torch.autograd.Function):
         y, last = _recurrence_forward(gate, x, state, reverse)
         ctx.reverse = reverse
         ctx.set_materialize_grads(False)
-        ctx.save_for_backward(gate, y if gate.requires_grad else None, state)
-        ctx.like = (x.shape, x.dtype, x.device)
+        ctx.save_for_backward(gate, y if ctx.needs_input_grad[0] else None, state)
         return y, last
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy, dlast):
-        gate, y, state = ctx.saved_tensors
-        shape, dtype, device = ctx.like
-        want_gate, want_x, want_state, _ = ctx.needs_input_grad
         if dy is None and dlast is None:
             return None, None, None, None
+        gate, y, state = ctx.saved_tensors
+        want_gate, want_x, want_state, _ = ctx.needs_input_grad
         if dy is None:
-            dy = torch.zeros(shape, dtype=dtype, device=device)
-        wide = _STATE_TYPE.get(dtype, torch.float32)
-        dstate = torch.empty((shape[0], shape[2]), dtype=wide, device=device) if want_state else None
+            dy = torch.zeros(gate.shape, dtype=gate.dtype, device=gate.device)
         if dlast is not None:
             dlast = dlast.contiguous()
+        B, T, D = dy.shape
+        dstate = dy.new_empty((B, D), dtype=_STATE_TYPE.get(dy.dtype, torch.float32)) if want_state else None
         if dy.numel() == 0:
-            return (torch.empty(shape, dtype=dtype, device=device) if want_gate else None,
-                    torch.empty(shape, dtype=dtype, device=device) if want_x else None,
-                    (torch.zeros_like(dstate) if dlast is None else dlast.clone()) if want_state else None, None)
-        channels = shape[2] > 1 and (dy.stride(2) == 1 or dy.stride(1) != 1)
+            return (torch.empty_like(dy) if want_gate else None, torch.empty_like(dy) if want_x else None,
+                    None if not want_state else torch.zeros_like(dstate) if dlast is None else dlast.clone(), None)
+        channels = D > 1 and (dy.stride(2) == 1 or dy.stride(1) != 1)
         gate, dy = _lined_up(gate, channels), _lined_up(dy, channels)
-        dx = _like(dy, channels)
-        dgate = None
+        dx, dgate = _like(dy, channels), None
         if want_gate:
             y, dgate = _lined_up(y, channels), _like(dy, channels)
-        _recurrence_call('mz_linear_recurrence_backward', gate, dy, state, ctx.reverse, dx, y=y if want_gate else None,
-                         out_gate=dgate, grad_last=dlast, out_state=dstate)
+        else:
+            y = None
+        _recurrence_call('mz_linear_recurrence_backward', gate, dy, state, ctx.reverse, dx, None, y, dgate, dlast, dstate)
         return dgate, dx if want_x else None, dstate, None
 
 
