@@ -433,7 +433,7 @@ typedef struct mz_strided {
  * out_gate = gradient of gate (both or neither; state as before); grad_last = gradient of last (NULL: 0), out_state =
  * gradient of state (may be NULL).  Inputs and outputs must not overlap. */
 typedef struct mz_recurrence {
-    int32_t type, B, D, reverse;
+    int32_t type, B, D, reverse;   /* B * D at most 2^30 */
     int64_t T;
     mz_strided gate, x, out, y, out_gate;
     const void *state;
@@ -462,7 +462,7 @@ int mz_linear_recurrence_backward(const mz_recurrence *args_h, void *stream);
 typedef struct mz_distill {
     int32_t type, teacher_type, index64;   /* MZ_F32 / MZ_BF16 / MZ_F16; 1 = index is int64, 0 = int32 */
     int32_t R, V, K;
-    float temperature;
+    float temperature;       /* 1e-30 .. 1e30 */
     const void *logits;      /* [R][V], rows logits_stride elements apart */
     int64_t logits_stride;
     const void *index;       /* [R][K] */
@@ -472,7 +472,7 @@ typedef struct mz_distill {
     const float *grad_loss;  /* [R] or NULL: 1 */
     float *loss;             /* [R] */
     void *grad;              /* [R][V], type of logits; must not overlap the logits */
-    float *stats;            /* [R][4] */
+    float *stats;            /* [R][4], aligned to 16 bytes */
 } mz_distill;
 int mz_distill_loss(const mz_distill *args_h, void *stream);
 int mz_distill_grad(const mz_distill *args_h, void *stream);

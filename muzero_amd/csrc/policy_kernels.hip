@@ -117,8 +117,8 @@ static int check_recurrence(const mz_recurrence *a, bool backward, const char *f
 {
     if (!a) return api_fail(MZ_ERR_ARG, std::string(fn) + ": null argument");
     if (a->type < MZ_F32 || a->type > MZ_F64) return api_fail(MZ_ERR_ARG, std::string(fn) + ": unknown element type");
-    if (a->B < 1 || a->D < 1 || a->T < 1 || (int64_t)a->B * a->D > INT32_MAX)
-        return api_fail(MZ_ERR_ARG, std::string(fn) + ": sizes must be positive, and B * D below 2^31");
+    if (a->B < 1 || a->D < 1 || a->T < 1 || (int64_t)a->B * a->D > (1 << 30))
+        return api_fail(MZ_ERR_ARG, std::string(fn) + ": sizes must be positive, and B * D at most 2^30");
     if (!a->gate.p || !a->x.p || !a->out.p) return api_fail(MZ_ERR_ARG, std::string(fn) + ": null tensor");
     if (backward && (a->out_gate.p != nullptr) != (a->y.p != nullptr))
         return api_fail(MZ_ERR_ARG, std::string(fn) + ": the gates' gradient needs the outputs, and nothing else does");
@@ -182,7 +182,8 @@ template <typename T, int G, int E, int MODE> static void launch_group(const Dis
 
 template <typename T, int THREADS, int NP, int MODE> static void launch_row(const DistillArgs &q, float c, hipStream_t st)
 {
-    const size_t lds = (size_t)q.K * (8 + 4 + 4) + (q.lse && MODE != 2 ? 4 * (((size_t)q.V + 8 + 31) / 32) : 0);
+    // entries, and with lse a bit for every action of whole packs (up to 14 more than there are actions)
+    const size_t lds = (size_t)q.K * (8 + 4 + 4) + (q.lse && MODE != 2 ? 4 * (((size_t)q.V + 16 + 31) / 32) : 0);
     hipLaunchKernelGGL((k_distill_row<T, THREADS, MODE == 1 ? NP : 0, MODE>), dim3((unsigned)q.R), dim3(THREADS), lds, st, q, c);
 }
 
@@ -208,12 +209,13 @@ template <int MODE> static int run_distill(const mz_distill *a, void *stream, co
     if (!a) return api_fail(MZ_ERR_ARG, std::string(fn) + ": null argument");
     if (a->type < MZ_F32 || a->type >= MZ_F64 || a->teacher_type < MZ_F32 || a->teacher_type >= MZ_F64)
         return api_fail(MZ_ERR_ARG, std::string(fn) + ": logits are float32, bfloat16 or float16");
-    if (a->R < 1 || a->V < 1 || a->K < 1 || a->K > MZ_DISTILL_MAX_ENTRIES || (a->lse && a->V > MZ_DISTILL_MAX_TAIL_ACTIONS))
+    if (a->R < 1 || a->V < 1 || a->V > (1 << 30) || a->K < 1 || a->K > MZ_DISTILL_MAX_ENTRIES || (a->lse && a->V > MZ_DISTILL_MAX_TAIL_ACTIONS))
         return api_fail(MZ_ERR_ARG, std::string(fn) + ": sizes outside the limits (entries 1.." + std::to_string(MZ_DISTILL_MAX_ENTRIES) +
                                         ", actions up to " + std::to_string(MZ_DISTILL_MAX_TAIL_ACTIONS) + " with lse)");
-    if (!(a->temperature > 0) || !std::isfinite(a->temperature)) return api_fail(MZ_ERR_ARG, std::string(fn) + ": temperature must be positive and finite");
+    if (!(a->temperature >= 1e-30f && a->temperature <= 1e30f)) return api_fail(MZ_ERR_ARG, std::string(fn) + ": temperature must lie in 1e-30 .. 1e30");
     if (!a->logits || !a->index || !a->teacher || (MODE != 2 && !a->loss) || (MODE != 0 && !a->grad) || (MODE != 1 && !a->stats))
         return api_fail(MZ_ERR_ARG, std::string(fn) + ": null tensor");
+    if ((uintptr_t)a->stats % 16) return api_fail(MZ_ERR_ARG, std::string(fn) + ": stats must be aligned to 16 bytes");
     DistillArgs q{};
     q.logits = a->logits, q.ld = a->logits_stride, q.index = a->index, q.teacher = a->teacher, q.lse = a->lse, q.weight = a->weight;
     q.up = MODE == 2 ? a->grad_loss : nullptr, q.loss = a->loss, q.grad = MODE ? a->grad : nullptr, q.stats = a->stats;

@@ -124,17 +124,17 @@ def _at(t):
 
 def _recurrence_call(what, gate, x, state, reverse, out, last=None, y=None, out_gate=None, grad_last=None, out_state=None):
     B, T, D = x.shape
+    if D == 1 and B > 1 and x.stride(0) == 1 and (T == 1 or x.stride(1) != 1):
+        # one channel, time-major (or a single position): the sequences are the channels of one
+        turned = [None if v is None else v.transpose(0, 2) for v in (gate, x, out, y, out_gate)]
+        if all(v is None or v.stride(2) == 1 for v in turned):
+            gate, x, out, y, out_gate = turned
+            B, D = 1, B
     if x.is_contiguous() and gate.is_contiguous() and out.is_contiguous() and (y is None or y.is_contiguous() and out_gate.is_contiguous()):
         n = T * D
         args = (_engine.ELEMENT_TYPES[x.dtype], B, D, reverse, T, gate.data_ptr(), n, D, 1, x.data_ptr(), n, D, 1,
                 out.data_ptr(), n, D, 1, _at(y), n, D, 1, _at(out_gate), n, D, 1, _at(state), _at(last), _at(grad_last), _at(out_state))
     else:
-        if D == 1 and T > 1 and x.stride(1) != 1 and x.stride(0) == 1:
-            # one channel, time-major: the rows are the channels of a single sequence
-            turned = [None if v is None else v.transpose(0, 2) for v in (gate, x, out, y, out_gate)]
-            if all(v is None or v.stride(2) == 1 for v in turned):
-                gate, x, out, y, out_gate = turned
-                B, D = 1, B
         args = (_engine.ELEMENT_TYPES[x.dtype], B, D, reverse, T, *_view(gate), *_view(x), *_view(out), *_view(y), *_view(out_gate),
                 _at(state), _at(last), _at(grad_last), _at(out_state))
     space, need = None, 0

@@ -138,6 +138,18 @@ def test_rows_of_no_weight_hold_anything():
         assert g.isfinite().all() and (g[0] == 0).all() and (g[2] == 0).all()
 
 
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('V,K', [(1, 70), (3, 100), (5, 1024), (300, 300), (17, 65), (2041, 66), (1009, 70)])
+def test_more_entries_than_lanes(V, K, dtype):
+    """Long lists of entries, most actions named several times, rows that begin anywhere in a pack of 16 bytes."""
+    g = torch.Generator().manual_seed(K)
+    logits = (torch.randn(7, V, generator=g) * 2).to(dtype).cuda()
+    index = torch.randint(-1, V + 1, (7, K), generator=g).int().cuda()
+    teacher = torch.randn(7, K, generator=g).to(dtype).cuda()
+    check(logits, index, teacher, None, 1.0, None)
+    check(logits, index, teacher, torch.full((7,), math.log(K) + 2.0).cuda(), 0.7, None)
+
+
 @pytest.mark.parametrize('V', [9, 500, 9000])
 def test_masked_logits(V):
     """Illegal actions at -inf or at the type's lowest value take no part; a teacher that names one gives an infinite loss."""
@@ -215,7 +227,75 @@ def test_trainer_distils_the_policy():
     before = [w.detach().clone() for w in net.parameters()]
     tr = Trainer(net, cfg)
     loss = tr.distill(obs, index, teacher)
-    assert abs(loss - float(plain)) <= 1e-5 * abs(float(plain)) + 1e-6 and tr.training_step == 1
+    assert abs(loss - float(plain.detach())) <= 1e-5 * abs(float(plain.detach())) + 1e-6 and tr.training_step == 1
     for w, b, grad in zip(net.parameters(), before, want):
         step = torch.zeros_like(b) if grad is None else cfg.lr * grad
         assert torch.allclose(w, b - step, rtol=1e-5, atol=1e-6)
+
+
+def test_offsets_beyond_32_bits():
+    """Rows whose distance in memory passes 2^31 elements."""
+    from muzero_amd.trainer import distillation_loss_grad
+    big = 2 ** 31 + 16
+    room = torch.empty(big + 200000, dtype=torch.bfloat16, device='cuda')
+    for V in (9, 700, 5000, 140000):
+        logits, index, teacher, _, _ = rows(2, V, 3, torch.bfloat16, V, 1.0, False, pad=False)
+        far = room.as_strided((2, V), (big, 1), 5)
+        far.copy_(logits)
+        loss, grad = distillation_loss_grad(far, index, teacher)
+        want = distillation_loss_grad(logits, index, teacher)
+        assert torch.allclose(loss, want[0], rtol=1e-5, atol=1e-6) and torch.allclose(grad, want[1], rtol=2.0 ** -7, atol=1e-9)
+
+
+def test_not_a_number_shows():
+    """A NaN logit makes its row NaN, whatever stands before it, and no other row."""
+    from muzero_amd.trainer import distillation_loss, distillation_loss_grad
+    for V in (9, 100, 800, 5000, 60000):
+        for at, low in ((0, False), (V - 1, False), (V // 2, True)):
+            logits, index, teacher, lse, _ = rows(3, V, 2, torch.bfloat16, V, 1.0, True, pad=False)
+            if low:
+                logits[1, :V // 2] = -math.inf
+            index[1] = torch.tensor([V - 2, V - 1])
+            logits[1, at] = math.nan
+            for tail in (lse, None):
+                leaf = logits.detach().requires_grad_()
+                total = distillation_loss(leaf, index, teacher, tail)
+                g, = torch.autograd.grad(total.sum(), leaf)
+                loss, grad = distillation_loss_grad(logits, index, teacher, tail)
+                for lo, gr in ((total, g), (loss, grad)):
+                    assert lo[1].isnan() and gr[1].isnan().all() and lo[[0, 2]].isfinite().all() and gr[[0, 2]].isfinite().all()
+
+
+def test_refusals():
+    from muzero_amd.engine import EngineError
+    from muzero_amd.trainer import distillation_loss, distillation_loss_grad
+    z, i, t = torch.zeros(4, 9, device='cuda'), torch.zeros(4, 2, dtype=torch.int64, device='cuda'), torch.zeros(4, 2, device='cuda')
+    f = torch.zeros(4, device='cuda')
+    for call in (distillation_loss, distillation_loss_grad):
+        for args in ((z[0], i, t), (z, i[0], t), (z, i[:3], t), (z, i, t[:, :1]), (z.double(), i, t), (z, i, t.double()), (z, i.short(), t),
+                     (z, i, t, f.double()), (z, i, t, f[:3]), (z, i, t, None, 1.0, f[:2]), (z, i, t, None, 0.0), (z, i, t, None, math.nan),
+                     (z, i[:, :0], t[:, :0]), (z, i.expand(2, 4, 2)[0].repeat(1, 600), t.repeat(1, 600))):
+            with pytest.raises(ValueError, match='distill'):
+                call(*args)
+        with pytest.raises(EngineError, match='device tensors'):
+            call(z, i.cpu(), t)
+        assert call(z[:0], i[:0], t[:0])[0].shape[0] == 0 if call is distillation_loss_grad else call(z[:0], i[:0], t[:0]).shape == (0,)
+    leaf = z.clone().requires_grad_()
+    g, = torch.autograd.grad(distillation_loss(leaf, i, t).sum(), leaf, create_graph=True)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(g.sum(), leaf)
+
+
+def test_two_streams_at_once():
+    from muzero_amd.trainer import distillation_loss_grad
+    args = [rows(300, 5000, 20, torch.bfloat16, s, 1.0, False)[:3] for s in (1, 2)]
+    want = [distillation_loss_grad(*a) for a in args]
+    streams, got = [torch.cuda.Stream() for _ in range(2)], []
+    for st in streams:
+        st.wait_stream(torch.cuda.current_stream())
+    for _ in range(3):
+        for st, a in zip(streams, args):
+            with torch.cuda.stream(st):
+                got.append(distillation_loss_grad(*a))
+    torch.cuda.synchronize()
+    assert all(torch.equal(g[0], want[k % 2][0]) and torch.equal(g[1], want[k % 2][1]) for k, g in enumerate(got))

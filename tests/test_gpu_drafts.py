@@ -149,3 +149,35 @@ def test_captured_and_replayed():
             want = verify_drafts(tokens, draft, target, ua, us)
             torch.cuda.synchronize()
             assert torch.equal(n, want[0]) and torch.equal(out, want[1])
+
+
+def test_offsets_beyond_32_bits():
+    big = 2 ** 31 + 8
+    room = torch.empty(2 * big + 300000, dtype=torch.bfloat16, device='cuda')
+    for V in (9, 100, 70000):
+        tokens, draft, target, ua, us = case(2, 1, V, torch.bfloat16, 4)
+        for strides in ((big, V, 1), (V, big, 1)):
+            far = room.as_strided((2, 2, V), strides, 3)
+            far.copy_(target)
+            check(tokens, draft, far, ua, us)
+            check(tokens, far[:, :1], target, ua, us)
+
+
+def test_refusals():
+    from muzero_amd.drafts import verify_drafts
+    from muzero_amd.engine import EngineError
+    tokens, draft, target, ua, us = case(3, 2, 9, torch.float32, 0)
+    n = torch.zeros(3, dtype=torch.int32).cuda()
+    for args in ((tokens[0], draft, target, ua, us), (tokens, draft[:, :1], target, ua, us), (tokens, draft, target[:, :2], ua, us),
+                 (tokens, draft.double(), target, ua, us), (tokens.float(), draft, target, ua, us), (tokens, draft, target, ua.float(), us),
+                 (tokens, draft, target, ua, us[:2]), (tokens, draft, target.int(), ua, us), (tokens, draft, target, ua, us, n.long()),
+                 (tokens, draft, target, ua, us, n[:2]), (tokens, draft[:, :, :0], target[:, :, :0], ua, us)):
+        with pytest.raises(ValueError, match='verify_drafts'):
+            verify_drafts(*args)
+    with pytest.raises(EngineError, match='device tensors'):
+        verify_drafts(tokens, draft.cpu(), target, ua, us)
+    wide = torch.zeros(1, 1, 1, dtype=torch.float16).cuda().expand(1, 1, (1 << 20) + 1)
+    with pytest.raises(ValueError, match='actions'):
+        verify_drafts(torch.zeros(1, 0, dtype=torch.int64).cuda(), None, wide, torch.zeros(1, 0, dtype=torch.float64).cuda(), us[:1])
+    n, out = verify_drafts(tokens[:0], draft[:0], target[:0], ua[:0], us[:0])
+    assert n.shape == (0,) and out.shape == (0, 3)

@@ -67,7 +67,7 @@ def close(got, want, z, T, dtype, extra=0.0):
 
 
 SHAPES = [(1, 1, 1), (3, 1, 5), (64, 1, 130), (2, 7, 64), (1, 255, 3), (5, 257, 33), (2, 1000, 66), (1, 129, 257), (300, 40, 1),
-          (7, 4097, 1), (1, 9001, 2), (3, 513, 128), (1, 2, 1000), (2, 128, 64), (1, 70000, 1)]
+          (7, 4097, 1), (1, 9001, 2), (3, 513, 128), (1, 2, 1000), (2, 128, 64), (1, 70000, 1), (5000, 1, 1), (999, 5, 1)]
 
 
 @pytest.mark.parametrize('dtype', TYPES)
@@ -253,3 +253,80 @@ def test_lambda_returns_of_a_move_log():
                     s = 1.0 if players[k, e] == players[k + 1, e] else -1.0
                     want[k, e] = r[k, e] + gamma * s * ((1 - lam) * v[k + 1, e] + lam * want[k + 1, e])
         np.testing.assert_allclose(got, want, rtol=0, atol=(6 * n + 8) * 2.0 ** -53 * 5 * n)
+
+
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('shape', [(1, 769, 3), (2, 1500, 130), (1, 3000, 66), (3, 2049, 40), (1, 6000, 514)])
+def test_chains_of_links(shape, dtype):
+    """Long records of few channels: right, the same bits every time, and so when two calls run at once on two streams."""
+    from muzero_amd.targets import linear_recurrence
+    B, T, D = shape
+    a, x, s = inputs(B, T, D, dtype, seed=T)
+    dy = torch.randn(B, T, D, generator=torch.Generator().manual_seed(1)).to(dtype).cuda()
+    for reverse in (False, True):
+        y_ref, last_ref = loop(a, x, s, reverse)
+        z, zl = loop(a.abs(), x.abs(), s.abs(), reverse)
+        y, last = linear_recurrence(a, x, s, reverse=reverse)
+        close(y, y_ref, z, T, dtype)
+        close(last, last_ref, zl, T, dtype)
+        leaves = [t.clone().requires_grad_() for t in (a, x, s)]
+        first = None
+        for _ in range(3):
+            y2, last2 = linear_recurrence(*leaves, reverse=reverse)
+            grads = torch.autograd.grad(y2, leaves, dy)
+            assert torch.equal(y, y2) and torch.equal(last, last2)
+            first = first or grads
+            assert all(torch.equal(g, f) for g, f in zip(grads, first))
+        dx_ref, _, ds_ref = loop_backward(a, y_ref, s, dy, None, reverse)
+        zx, _, zs = loop_backward(a.abs(), z, s.abs(), dy.abs(), None, reverse)
+        close(first[1], dx_ref, zx, T, dtype)
+        close(first[2], ds_ref, zs, T + 1, dtype)
+        streams, outs = [torch.cuda.Stream() for _ in range(2)], []
+        for st in streams:
+            st.wait_stream(torch.cuda.current_stream())
+        for _ in range(3):
+            for st in streams:
+                with torch.cuda.stream(st):
+                    outs.append(linear_recurrence(a, x, s, reverse=reverse))
+        for st in streams:
+            torch.cuda.current_stream().wait_stream(st)
+        assert all(torch.equal(o, y) and torch.equal(l, last) for o, l in outs)
+
+
+def test_offsets_beyond_32_bits():
+    """Sequences, positions and channels whose distance in memory passes 2^31 elements."""
+    from muzero_amd.targets import linear_recurrence
+    big = 2 ** 31 + 64
+    room = torch.empty(2 * big + 70000, dtype=torch.bfloat16, device='cuda')
+    for shape, strides in (((2, 300, 64), (big, 64, 1)), ((2, 3, 64), (big, 64, 1)), ((1, 3, 64), (0, big, 1)), ((2, 1000, 8), (big, 8, 1)),
+                           ((2, 700, 1), (big, 1, 1)), ((1, 500, 3), (0, 1, big))):
+        B, T, D = shape
+        a, x, _ = inputs(B, T, D, torch.bfloat16, seed=T)
+        far = room.as_strided(shape, strides, 8)
+        far.copy_(x)
+        y, last = linear_recurrence(a, far)
+        y_ref, last_ref = loop(a, x, None, False)
+        z, zl = loop(a.abs(), x.abs(), None, False)
+        close(y, y_ref, z, T, torch.bfloat16)
+        close(last, last_ref, zl, T, torch.bfloat16)
+
+
+def test_refusals():
+    from muzero_amd.targets import linear_recurrence
+    t = torch.zeros(2, 3, 4, device='cuda')
+    s = torch.zeros(2, 4, device='cuda')
+    for args in ((t[0], t[0]), (t, t[:1]), (t, t.half()), (t.int(), t.int()), (t, t, s.double()), (t, t, s[:1]), (t, t, s.cpu()),
+                 (t.half(), t.half(), s.half()), (t.double(), t.double(), s)):
+        with pytest.raises(ValueError, match='linear_recurrence'):
+            linear_recurrence(*args)
+    x = t.clone().requires_grad_()
+    y, _ = linear_recurrence(t, x)
+    g, = torch.autograd.grad(y.sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(g.sum(), x)                 # differentiable once
+    gate = t.clone().requires_grad_()
+    y, _ = linear_recurrence(gate, x)
+    with torch.no_grad():
+        y.add_(1.0)
+    with pytest.raises(RuntimeError, match='modified by an inplace operation'):
+        torch.autograd.grad(y.sum(), gate)
