@@ -44,19 +44,6 @@ __device__ __forceinline__ int entry_at(const DistillArgs &q, long long i)
 
 
 
-template <int G> __device__ __forceinline__ double group_sum(double v)
-{
-#pragma unroll
-    for (int k = G / 2; k; k /= 2) v += __shfl_xor(v, k);
-    return v;
-}
-template <int G> __device__ __forceinline__ float group_max(float v)
-{
-#pragma unroll
-    for (int k = G / 2; k; k /= 2) v = fmaxf(v, __shfl_xor(v, k));
-    return v;
-}
-
 // What a row's entries come to: their probabilities' sum, sum p log p, and what the teacher has left.
 struct Mass { double mass, ent, rest; bool some; };
 
@@ -152,20 +139,31 @@ __global__ __launch_bounds__(256) void k_distill_group(DistillArgs q, float c)
         }
         return;
     }
-    // which of the lane's actions are entries, and what all entries of the same action come to
+    // which of the lane's actions are entries; an action that several entries name gets their sum, at the first of them
     unsigned inside = 0;
     double total[C];
     bool first[C];
 #pragma unroll
-    for (int i = 0; i < C; i++) total[i] = 0, first[i] = index[i] >= 0;
+    for (int i = 0; i < C; i++) total[i] = p[i], first[i] = index[i] >= 0;
     if (MODE != 0 || q.lse) {
+        bool again = false;
 #pragma unroll
         for (int i = 0; i < C; i++)
             for (int l = 0; l < G; l++) {
                 if (l + i * G >= q.K) break;
                 const int j = __shfl(index[i], l, G);
                 if (j >= 0 && j % G == lane) inside |= 1u << (j / G);
-                if (MODE != 0) {
+#pragma unroll
+                for (int c = 0; c < C; c++) again |= index[c] == j && j >= 0 && l + i * G < lane + c * G;
+            }
+        if (MODE != 0 && __any(again)) {
+#pragma unroll
+            for (int c = 0; c < C; c++) total[c] = 0;
+#pragma unroll
+            for (int i = 0; i < C; i++)
+                for (int l = 0; l < G; l++) {
+                    if (l + i * G >= q.K) break;
+                    const int j = __shfl(index[i], l, G);
                     const double pj = __shfl(p[i], l, G);
 #pragma unroll
                     for (int c = 0; c < C; c++) {
@@ -173,7 +171,7 @@ __global__ __launch_bounds__(256) void k_distill_group(DistillArgs q, float c)
                         if (index[c] == j && l + i * G < lane + c * G) first[c] = false;
                     }
                 }
-            }
+        }
     }
     float m;
     double dsum, dtail;
@@ -189,7 +187,7 @@ __global__ __launch_bounds__(256) void k_distill_group(DistillArgs q, float c)
             sum += x;
             if (q.lse && !(inside >> i & 1)) tail += x;
         }
-        dsum = group_sum<G>(sum), dtail = group_sum<G>(tail);
+        dsum = group_sum<G>((double)sum), dtail = group_sum<G>((double)tail);
         if (dtail == 0) e.rest = 0;   // no action outside the entries has anything left
         const double lsum = log(dsum), inv_tau = 1.0 / (double)q.tau;
         double cross = 0;
@@ -457,7 +455,7 @@ __global__ __launch_bounds__(THREADS, NP == 16 ? 4 : NP ? 6 : 1) void k_distill_
         const float down = own == -HUGE_VALF ? 1.0f : expo(own - m, c);
         sum *= down, tail *= down;
         if (m == -HUGE_VALF) sum = tail = m - m;   // no logit above -inf: not a number
-        dsum = group_sum<64>(sum), dtail = group_sum<64>(tail);
+        dsum = group_sum<64>((double)sum), dtail = group_sum<64>((double)tail);
         if (lane == 0) red[0][w] = dsum, red[1][w] = dtail;
         __syncthreads();
         dsum = dtail = 0;

@@ -25,6 +25,46 @@ __device__ __forceinline__ void lds_fence_barrier()
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
 }
 
+// Value of another lane of the same 16 by a register move (0 where there is none): a few cycles, against about a hundred for a
+// shuffle through LDS.
+template <int CTRL> __device__ __forceinline__ float lane_move(float v)
+{
+    return __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), CTRL, 0xF, 0xF, true));
+}
+template <int CTRL> __device__ __forceinline__ double lane_move(double v)
+{
+    const long long b = __builtin_bit_cast(long long, v);
+    const int lo = __builtin_amdgcn_mov_dpp((int)b, CTRL, 0xF, 0xF, true), hi = __builtin_amdgcn_mov_dpp((int)(b >> 32), CTRL, 0xF, 0xF, true);
+    return __builtin_bit_cast(double, (long long)hi << 32 | (unsigned)lo);
+}
+__device__ __forceinline__ float lane_read(float v, int lane) { return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), lane)); }
+__device__ __forceinline__ double lane_read(double v, int lane)
+{
+    const long long b = __builtin_bit_cast(long long, v);
+    return __builtin_bit_cast(double, (long long)__builtin_amdgcn_readlane((int)(b >> 32), lane) << 32 | (unsigned)__builtin_amdgcn_readlane((int)b, lane));
+}
+// f over G neighbouring lanes (4, 16 or 64, all of them at work), in every one of them, always in the same order.
+template <int G, typename V, typename F> __device__ __forceinline__ V group_fold(V v, F f)
+{
+    static_assert(G == 4 || G == 16 || G == 64, "groups of 4, 16 or 64 lanes");
+    v = f(v, lane_move<0xB1>(v));    // lanes 1, 0, 3, 2 of every four
+    v = f(v, lane_move<0x4E>(v));    // lanes 2, 3, 0, 1
+    if constexpr (G > 4) {
+        v = f(v, lane_move<0x141>(v));   // mirrored in every eight
+        v = f(v, lane_move<0x140>(v));   // mirrored in every sixteen
+    }
+    if constexpr (G == 64) v = f(f(lane_read(v, 0), lane_read(v, 16)), f(lane_read(v, 32), lane_read(v, 48)));
+    return v;
+}
+template <int G, typename V> __device__ __forceinline__ V group_sum(V v)
+{
+    return group_fold<G>(v, [](V a, V b) { return a + b; });
+}
+template <int G> __device__ __forceinline__ float group_max(float v)
+{
+    return group_fold<G>(v, [](float a, float b) { return fmaxf(a, b); });
+}
+
 // N elements that travel as one load or store; aligned to its size.
 template <typename T, int N> struct alignas(sizeof(T) * N) Pack { T v[N]; };
 // ... aligned to one element only (one wide access all the same: gfx950 takes any element-aligned address).

@@ -193,8 +193,6 @@ template <typename T, int MODE> static void launch_distill(const DistillArgs &q,
     const int packs = (q.V + W - 1) / W + 1;   // one more where a row begins inside a pack
     if (q.V <= 16 && q.K <= 16) launch_group<T, 4, 4, MODE>(q, c, st);
     else if (q.V <= 64 && q.K <= 64) launch_group<T, 16, 4, MODE>(q, c, st);
-    else if (q.V <= 256 && q.K <= 64) launch_group<T, 64, 4, MODE>(q, c, st);
-    else if (q.V <= 1024 && q.K <= 64) launch_group<T, 64, 16, MODE>(q, c, st);
     else if (packs <= 64 * 8) launch_row<T, 64, 8, MODE>(q, c, st);
     else if (packs <= 128 * 8) launch_row<T, 128, 8, MODE>(q, c, st);
     else if (packs <= 256 * 8) launch_row<T, 256, 8, MODE>(q, c, st);

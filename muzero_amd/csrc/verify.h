@@ -214,8 +214,7 @@ template <typename T> __global__ __launch_bounds__(1024) void k_verify(VerifyArg
             for (int a = 0; a < 4; a++)
 #pragma unroll
                 for (int e = 0; e < E; e++) s += v[a][e];
-#pragma unroll
-            for (int k = 32; k; k /= 2) s += __shfl_xor(s, k);
+            s = group_sum<64>(s);
             if (lane == 0) part[i] = s;
         }
         __syncthreads();
