@@ -28,6 +28,7 @@ struct DistillArgs {
     int R, V, K;
     int index64, teacher_type;
     float tau;
+    double inv_tau;
 };
 
 __device__ __forceinline__ float teacher_at(const DistillArgs &q, long long i)
@@ -44,14 +45,27 @@ __device__ __forceinline__ int entry_at(const DistillArgs &q, long long i)
 
 
 
-// What a row's entries come to: their probabilities' sum, sum p log p, and what the teacher has left.
-struct Mass { double mass, ent, rest; bool some; };
+// What a row's entries come to: sum p, sum p u with p = exp(u) / norm, the norm, and what the teacher has left.
+struct Mass { double mass, ent, norm, rest; bool some; };
 
-// G lanes, C entries each: action, teacher's logit -> probability p and log p.  An absent entry has action -1 and p = 0.
+// From the sums over unnormalised p.
+__device__ __forceinline__ void settle(const DistillArgs &q, Mass &e)
+{
+    const double sum = e.norm;
+    if (q.lse) {
+        e.mass = sum, e.norm = 1.0;
+        e.rest = sum != sum ? sum : fmax(1.0 - sum, 0.0);
+    } else {
+        e.mass = sum == 0 ? 0.0 : sum != sum ? sum : 1.0;
+        e.ent = sum == 0 ? 0.0 : e.ent / sum;
+        e.rest = 0.0;
+    }
+}
+
+// G lanes, C entries each: action, teacher's logit -> probability p.  An absent entry has action -1 and p = 0.
 template <int G, int C>
 __device__ __forceinline__ Mass weigh(const DistillArgs &q, long long row, const int (&index)[C], const float (&t)[C], double (&p)[C])
 {
-    const double inv_tau = 1.0 / (double)q.tau;
     float top = -HUGE_VALF;
     bool any = false;
 #pragma unroll
@@ -61,31 +75,22 @@ __device__ __forceinline__ Mass weigh(const DistillArgs &q, long long row, const
     }
     Mass e;
     e.some = group_max<G>(any ? 1.0f : 0.0f) != 0.0f;
-    double logp[C], sum = 0;
-    if (q.lse) {
-        const double lse = q.lse[row];
-#pragma unroll
-        for (int i = 0; i < C; i++) logp[i] = (double)t[i] * inv_tau - lse;
-    } else {
-        top = group_max<G>(top);
-#pragma unroll
-        for (int i = 0; i < C; i++) logp[i] = ((double)t[i] - (double)top) * inv_tau;
-    }
-#pragma unroll
-    for (int i = 0; i < C; i++) p[i] = t[i] == -HUGE_VALF ? 0.0 : exp(logp[i]), sum += p[i];
-    sum = group_sum<G>(sum);
-    const double norm = q.lse ? 1.0 : 1.0 / sum, shift = q.lse ? 0.0 : log(sum);
-    double ent = 0;
+    const double from = q.lse ? (double)q.lse[row] : (double)group_max<G>(top) * q.inv_tau;
+    double sum = 0, ent = 0;
 #pragma unroll
     for (int i = 0; i < C; i++) {
-        if (p[i] == 0) continue;
-        p[i] *= norm;
-        ent += p[i] * (logp[i] - shift);
+        const double u = (double)t[i] * q.inv_tau - from;
+        p[i] = t[i] == -HUGE_VALF ? 0.0 : exp(u);
+        sum += p[i];
+        if (!(p[i] == 0)) ent += p[i] * u;
     }
-    e.ent = group_sum<G>(ent);
-    e.mass = q.lse ? sum : sum > 0 || sum != sum ? sum * norm : 0.0;
-    e.rest = q.lse ? fmax(1.0 - sum, 0.0) : 0.0;
-    if (sum != sum) e.rest = sum;
+    e.norm = group_sum<G>(sum), e.ent = group_sum<G>(ent);
+    settle(q, e);
+    if (!q.lse) {
+        const double scale = 1.0 / e.norm;
+#pragma unroll
+        for (int i = 0; i < C; i++) p[i] = p[i] == 0 ? 0.0 : p[i] * scale;
+    }
     return e;
 }
 
@@ -93,11 +98,14 @@ __device__ __forceinline__ Mass weigh(const DistillArgs &q, long long row, const
 // temperature by 2^-25 of itself, and a -inf logit stays at 0.
 __device__ __forceinline__ float expo(float d, float c) { return __builtin_amdgcn_exp2f(d * c); }
 
-__device__ __forceinline__ double divergence(const Mass &e, double cross, double dsum, double dtail)
+// The divergence, in lane 0 of G: cross = sum p (z - m) / tau; dsum, dtail: sums of the student's exponentials over all
+// actions and over those outside the entries.  Three logarithms, taken by three lanes at once.
+template <int G>
+__device__ __forceinline__ double divergence(const Mass &e, double cross, double dsum, double ratio, int lane)
 {
-    double kl = e.ent - cross;
-    if (!(e.rest == 0)) kl += e.rest * (log(e.rest) - log(dtail) + log(dsum));
-    return kl;
+    const double l = log(lane == 1 ? dsum : lane == 2 && !(e.rest == 0) ? ratio : lane == 0 && e.norm > 0 ? e.norm : 1.0);
+    const double of_sum = __shfl(l, 1, G), of_ratio = __shfl(l, 2, G);   // of_ratio: of rest dsum / dtail
+    return e.ent - e.mass * l - (cross - e.mass * of_sum) + (e.rest == 0 ? 0.0 : e.rest * of_ratio);
 }
 
 // Small action sets: G lanes of a wave hold a row, E actions and 4 entries a lane, all of it in registers.  MODE 0: loss and
@@ -188,15 +196,15 @@ __global__ __launch_bounds__(256) void k_distill_group(DistillArgs q, float c)
             if (q.lse && !(inside >> i & 1)) tail += x;
         }
         dsum = group_sum<G>((double)sum), dtail = group_sum<G>((double)tail);
-        if (dtail == 0) e.rest = 0;   // no action outside the entries has anything left
-        const double lsum = log(dsum), inv_tau = 1.0 / (double)q.tau;
         double cross = 0;
 #pragma unroll
         for (int i = 0; i < C; i++)
-            if (!(p[i] == 0)) cross += p[i] * (((double)ze[i] - (double)m) * inv_tau - lsum);
+            if (!(p[i] == 0)) cross += p[i] * (((double)ze[i] - (double)m) * q.inv_tau);
         cross = group_sum<G>(cross);
+        if (dtail == 0) e.rest = 0;   // no action outside the entries has anything left
+        const double kl = divergence<G>(e, cross, dsum, e.rest == 0 ? 1.0 : e.rest * dsum / dtail, lane);
         if (lane == 0) {
-            q.loss[row] = (float)((double)weight * q.tau * q.tau * divergence(e, cross, dsum, dtail));
+            q.loss[row] = (float)((double)weight * q.tau * q.tau * kl);
             if (MODE == 0) *(float4 *)(q.stats + row * 4) = make_float4(m, (float)dsum, (float)dtail, 1.0f);
         }
     } else {
@@ -205,8 +213,8 @@ __global__ __launch_bounds__(256) void k_distill_group(DistillArgs q, float c)
         if (dtail == 0) e.rest = 0;
     }
     if (MODE == 0) return;
-    const double whole = e.mass + e.rest, outside = e.rest == 0 ? whole : whole - e.rest * dsum / dtail;
-    const float f = (float)(outside / dsum * scale), fi = (float)(whole / dsum * scale);
+    const double whole = e.mass + e.rest, outside = e.rest == 0 ? whole : whole - e.rest * dsum / dtail, per = (double)scale / dsum;
+    const float f = (float)(outside * per), fi = (float)(whole * per);
 #pragma unroll
     for (int i = 0; i < E; i++) {
         const int j = lane + i * G;
@@ -251,7 +259,7 @@ __global__ __launch_bounds__(THREADS, NP == 16 ? 4 : NP ? 6 : 1) void k_distill_
     extern __shared__ double lds[];
     __shared__ double red[2][NW];
     __shared__ float red_m[NW];
-    __shared__ double share[3];
+    __shared__ double share[4];
     __shared__ int share_some, repeated;
     double *ep = lds;                                     // [K] probability of an entry
     float *ez = (float *)(lds + q.K);                     // [K] the student's logit of its action
@@ -340,9 +348,8 @@ __global__ __launch_bounds__(THREADS, NP == 16 ? 4 : NP ? 6 : 1) void k_distill_
             if (lane < q.K) put(lane, index[0]);
             const Mass e = weigh<64, 1>(q, row, index, t, p);
             if (lane < q.K) ep[lane] = p[0];
-            if (lane == 0) share[0] = e.mass, share[1] = e.ent, share[2] = e.rest, share_some = e.some;
+            if (lane == 0) share[0] = e.mass, share[1] = e.ent, share[2] = e.norm, share[3] = e.rest, share_some = e.some;
         } else {   // in rounds of 64, over lists in LDS
-            const double inv_tau = 1.0 / (double)q.tau;
             float top = -HUGE_VALF;
             bool some = false;
             for (int k = lane; k < q.K; k += 64) {
@@ -353,23 +360,22 @@ __global__ __launch_bounds__(THREADS, NP == 16 ? 4 : NP ? 6 : 1) void k_distill_
                 some |= j >= 0;
                 top = fmaxf(top, t);
             }
-            const double from = q.lse ? (double)q.lse[row] : (double)group_max<64>(top) * inv_tau;
+            const double from = q.lse ? (double)q.lse[row] : (double)group_max<64>(top) * q.inv_tau;
             double total = 0, ent = 0;
-            for (int k = lane; k < q.K; k += 64) total += ep[k] == -HUGE_VAL ? 0.0 : exp(ep[k] * inv_tau - from);
-            total = group_sum<64>(total);
-            const double norm = q.lse ? 1.0 : 1.0 / total, less = q.lse ? 0.0 : log(total);
             for (int k = lane; k < q.K; k += 64) {
-                const double u = ep[k] * inv_tau - from, x = ep[k] == -HUGE_VAL ? 0.0 : exp(u) * norm;
+                const double u = ep[k] * q.inv_tau - from, x = ep[k] == -HUGE_VAL ? 0.0 : exp(u);
                 ep[k] = x;
-                if (!(x == 0)) ent += x * (u - less);
+                total += x;
+                if (!(x == 0)) ent += x * u;
             }
-            ent = group_sum<64>(ent);
-            some = __any(some);
-            if (lane == 0) {
-                share[0] = q.lse ? total : total == 0 ? 0.0 : total * norm, share[1] = ent;
-                share[2] = q.lse ? (total != total ? total : fmax(1.0 - total, 0.0)) : 0.0;
-                share_some = some;
+            Mass e;
+            e.norm = group_sum<64>(total), e.ent = group_sum<64>(ent), e.some = __any(some);
+            settle(q, e);
+            if (!q.lse) {
+                const double scale_p = 1.0 / e.norm;
+                for (int k = lane; k < q.K; k += 64) ep[k] = ep[k] == 0 ? 0.0 : ep[k] * scale_p;
             }
+            if (lane == 0) share[0] = e.mass, share[1] = e.ent, share[2] = e.norm, share[3] = e.rest, share_some = e.some;
         }
         begin();
     } else begin();   // the other waves' first packs are on their way meanwhile
@@ -397,7 +403,7 @@ __global__ __launch_bounds__(THREADS, NP == 16 ? 4 : NP ? 6 : 1) void k_distill_
         return t;
     };
     __syncthreads();
-    Mass e{share[0], share[1], share[2], share_some != 0};
+    Mass e{share[0], share[1], share[2], share[3], share_some != 0};
     if (!e.some) {
         nothing();
         return;
@@ -464,12 +470,12 @@ __global__ __launch_bounds__(THREADS, NP == 16 ? 4 : NP ? 6 : 1) void k_distill_
         if (dtail == 0) e.rest = 0;   // no action outside the entries has anything left
         if (w == NW - 1) {
             double cross = 0;
-            const double lsum = log(dsum), inv_tau = 1.0 / (double)q.tau;
             for (int k = lane; k < q.K; k += 64)
-                if (!(ep[k] == 0)) cross += ep[k] * (((double)ez[k] - (double)m) * inv_tau - lsum);
+                if (!(ep[k] == 0)) cross += ep[k] * (((double)ez[k] - (double)m) * q.inv_tau);
             cross = group_sum<64>(cross);
+            const double kl = divergence<64>(e, cross, dsum, e.rest == 0 ? 1.0 : e.rest * dsum / dtail, lane);
             if (lane == 0) {
-                q.loss[row] = (float)((double)weight * q.tau * q.tau * divergence(e, cross, dsum, dtail));
+                q.loss[row] = (float)((double)weight * q.tau * q.tau * kl);
                 if (MODE == 0) *(float4 *)(q.stats + row * 4) = make_float4(m, (float)dsum, (float)dtail, 1.0f);
             }
         }
@@ -480,8 +486,8 @@ __global__ __launch_bounds__(THREADS, NP == 16 ? 4 : NP ? 6 : 1) void k_distill_
     }
     if (MODE == 0) return;
     // q_j times what stands outside the entries; the entries themselves are put right behind the barrier
-    const double whole = e.mass + e.rest, outside = e.rest == 0 ? whole : whole - e.rest * dsum / dtail;
-    const float f = (float)(outside / dsum * scale), fi = (float)(whole / dsum * scale);
+    const double whole = e.mass + e.rest, outside = e.rest == 0 ? whole : whole - e.rest * dsum / dtail, per = (double)scale / dsum;
+    const float f = (float)(outside * per), fi = (float)(whole * per);
     for (int k = tid; k < q.K; k += THREADS) {
         bool other = false;
         for (int i = 0; i < q.K; i++) other |= i != k && ei[i] == ei[k];

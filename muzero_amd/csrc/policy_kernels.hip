@@ -193,6 +193,8 @@ template <typename T, int MODE> static void launch_distill(const DistillArgs &q,
     const int packs = (q.V + W - 1) / W + 1;   // one more where a row begins inside a pack
     if (q.V <= 16 && q.K <= 16) launch_group<T, 4, 4, MODE>(q, c, st);
     else if (q.V <= 64 && q.K <= 64) launch_group<T, 16, 4, MODE>(q, c, st);
+    else if (packs <= 64 * 2) launch_row<T, 64, 2, MODE>(q, c, st);
+    else if (packs <= 64 * 4) launch_row<T, 64, 4, MODE>(q, c, st);
     else if (packs <= 64 * 8) launch_row<T, 64, 8, MODE>(q, c, st);
     else if (packs <= 128 * 8) launch_row<T, 128, 8, MODE>(q, c, st);
     else if (packs <= 256 * 8) launch_row<T, 256, 8, MODE>(q, c, st);
@@ -217,7 +219,7 @@ template <int MODE> static int run_distill(const mz_distill *a, void *stream, co
     DistillArgs q{};
     q.logits = a->logits, q.ld = a->logits_stride, q.index = a->index, q.teacher = a->teacher, q.lse = a->lse, q.weight = a->weight;
     q.up = MODE == 2 ? a->grad_loss : nullptr, q.loss = a->loss, q.grad = MODE ? a->grad : nullptr, q.stats = a->stats;
-    q.R = a->R, q.V = a->V, q.K = a->K, q.index64 = a->index64, q.teacher_type = a->teacher_type, q.tau = a->temperature;
+    q.R = a->R, q.V = a->V, q.K = a->K, q.index64 = a->index64, q.teacher_type = a->teacher_type, q.tau = a->temperature, q.inv_tau = 1.0 / (double)a->temperature;
     const float c = (float)(1.4426950408889634074 / (double)a->temperature);   // log2(e) / temperature
     hipStream_t st = (hipStream_t)stream;
     switch (a->type) {
