@@ -443,7 +443,7 @@ typedef struct mz_recurrence {
     void *workspace;           /* device memory of this call alone, 64-byte aligned, or NULL where none is needed */
     int64_t workspace_bytes;
 } mz_recurrence;
-/* Device bytes a call with these arguments needs as workspace (often 0; backward != 0: of the backward call). */
+/* Device bytes a call with these arguments needs as workspace (0 up to T = 256; backward != 0: of the backward call). */
 int mz_linear_recurrence_workspace(const mz_recurrence *args_h, int32_t backward, int64_t *out_bytes);
 int mz_linear_recurrence(const mz_recurrence *args_h, void *stream);
 int mz_linear_recurrence_backward(const mz_recurrence *args_h, void *stream);

@@ -254,7 +254,7 @@ template <> __device__ __forceinline__ unsigned lowest_bits<_Float16>() { return
 // maximum per thread, the gradient another; the loss and gradient pass keeps rows of up to NP packs a thread in registers
 // between the two (NP > 0) and reads wider ones again.
 // 4096 x 32000 bfloat16, 32 entries, loss and gradient: 116 us (524 MB, 4.5 TB/s; a copy 5.1).  1023 x 131071, 64 entries and the
-// remaining mass: loss 85 us (268 MB, 3.2 TB/s: 4 rows a compute unit, whose first and last steps overlap little), gradient 105 us
+// remaining mass: loss 76 us (268 MB, 3.5 TB/s: 4 rows a compute unit, whose first and last steps overlap little), gradient 106 us
 // (536 MB, 5.1 TB/s).  Short rows are bound by the entries' float64 arithmetic: 40000 x 200 in 55 us.
 template <typename T, int THREADS, int NP, int MODE>
 __global__ __launch_bounds__(THREADS, NP == 16 ? 4 : NP ? 6 : 1) void k_distill_row(DistillArgs q, float c)

@@ -23,9 +23,11 @@ static size_t size_of(int type) { return type == MZ_F64 ? 8 : type == MZ_F32 ? 4
 // - From REC_MANY_TILES tiles on a strand is 64 lanes wide, 256 bytes of a position: 32 x 2048 x 4096 bfloat16 330 against 367 us.
 // - Below REC_FEW_TILES tiles of 32 lanes, records of REC_LEAST_LINKS links or more are cut into chains: 1 x 4096 x 512 bfloat16
 //   14 against 49 us, 4 x 2048 x 1024 19 against 32, 6 x 2048 x 2048 (192 tiles) 40 against 46, at 256 tiles 109 against 102;
-//   three links (1 x 600 x 512) 11.2 against 10.5, their gradients 15.3 against 17.6.
+//   three links (1 x 600 x 512) 11.2 against 10.5, their gradients 15.3 against 17.6.  Gradients, with five tensors on their
+//   way, gain up to REC_FEW_TILES_BACKWARD tiles: 4 x 8192 x 4096 (256 tiles) 301 against 334, 8 x 2048 x 2500 (320) 114
+//   against 159.
 constexpr int REC_LENGTH = 8;
-constexpr long long REC_MANY_TILES = 512, REC_FEW_TILES = 256, REC_LEAST_LINKS = 3;
+constexpr long long REC_MANY_TILES = 512, REC_FEW_TILES = 256, REC_FEW_TILES_BACKWARD = 512, REC_LEAST_LINKS = 3;
 
 // How a recurrence is run: chosen by sizes, strides and alignment alone, for the workspace query and the call alike.
 struct RecurrencePlan {
@@ -35,7 +37,7 @@ struct RecurrencePlan {
 };
 
 // VEC = 2 is a 4-byte access of a 16-bit type
-static RecurrencePlan plan_recurrence(const mz_recurrence *a)
+static RecurrencePlan plan_recurrence(const mz_recurrence *a, bool backward)
 {
     RecurrencePlan p{true, false, 1, 32, 1, 0};
     uint64_t low = 0;   // low bits of every address and step along the axis and the sequences
@@ -60,8 +62,8 @@ static RecurrencePlan plan_recurrence(const mz_recurrence *a)
     auto tiles_of = [&](int lanes) { return (long long)a->B * ((a->D + lanes * p.vec - 1) / (lanes * p.vec)); };
     p.lanes = tiles_of(64) >= REC_MANY_TILES ? 64 : 32;
     p.strands = (int)std::min<long long>(REC_THREADS / p.lanes, std::max<long long>(2, (a->T + REC_LENGTH - 1) / REC_LENGTH));
-    const long long links = (a->T + CHAIN_ROWS(size) - 1) / CHAIN_ROWS(size);
-    if (tiles_of(32) < REC_FEW_TILES && links >= REC_LEAST_LINKS && links * tiles_of(64) < INT32_MAX) p.links = (int)links;
+    const long long links = (a->T + CHAIN_ROWS(size, backward) - 1) / CHAIN_ROWS(size, backward);
+    if (a->T > 256 && tiles_of(32) < (backward ? REC_FEW_TILES_BACKWARD : REC_FEW_TILES) && links >= REC_LEAST_LINKS && links * tiles_of(64) < INT32_MAX) p.links = (int)links;
     return p;
 }
 
@@ -82,7 +84,7 @@ template <typename T, int VEC, bool BWD> static void launch_chain(const Recurren
     const unsigned blocks = (unsigned)std::min<long long>((granules + 255) / 256, 2048);
     hipLaunchKernelGGL(k_zero_granules, dim3(blocks), dim3(256), 0, st, q.granules, granules);
     const long long tiles = (long long)q.B * ((q.D + 64 * VEC - 1) / (64 * VEC));
-    hipLaunchKernelGGL((k_recurrence_chain<T, VEC, BWD>), dim3((unsigned)(tiles * q.links)), dim3(64 * CHAIN_WAVES), 0, st, q);
+    hipLaunchKernelGGL((k_recurrence_chain<T, VEC, BWD>), dim3((unsigned)(tiles * q.links)), dim3(64 * CHAIN_WAVES(sizeof(T), BWD)), 0, st, q);
 }
 
 template <typename T, int VEC, bool BWD> static void launch_channels(const RecurrencePlan &p, const RecurrenceArgs &q, hipStream_t st)
@@ -136,7 +138,7 @@ template <bool BWD> static int run_recurrence(const mz_recurrence *a, void *stre
 {
     (void)hipGetLastError();
     if (int rc = check_recurrence(a, BWD, fn)) return rc;
-    const RecurrencePlan p = plan_recurrence(a);
+    const RecurrencePlan p = plan_recurrence(a, BWD);
     if (p.links && (a->workspace_bytes < (int64_t)(8 * granule_count(a, p)) || !a->workspace || (uintptr_t)a->workspace % 64))
         return api_fail(MZ_ERR_ARG, std::string(fn) + ": the workspace is smaller than mz_linear_recurrence_workspace says, or not aligned to 64 bytes");
     RecurrenceArgs q{};
@@ -175,7 +177,7 @@ extern "C" int mz_linear_recurrence_workspace(const mz_recurrence *args_h, int32
 {
     if (int rc = check_recurrence(args_h, backward != 0, "mz_linear_recurrence_workspace")) return rc;
     if (!out_bytes) return api_fail(MZ_ERR_ARG, "mz_linear_recurrence_workspace: null argument");
-    *out_bytes = (int64_t)(8 * granule_count(args_h, plan_recurrence(args_h)));
+    *out_bytes = (int64_t)(8 * granule_count(args_h, plan_recurrence(args_h, backward != 0)));
     return MZ_OK;
 }
 
@@ -200,7 +202,8 @@ template <typename T, int MODE> static void launch_distill(const DistillArgs &q,
     // groups of a whole wave took 125, the block 55).  Then as few waves a row as keep its packs in registers: 6000 bfloat16 in 78 us
     // with 128 threads of 8 packs, 89 with 64 of 16; 32000 in 118 with 256 of 16, 131 with 512 of 8, 165 with 1024 of 4, 141 read
     // twice; 1000 float32 in 38 with 4 packs a thread, 45 with 8 (idle packs cost exponentials).  Wider rows are read twice:
-    // 131071 in 165, 183 where 1024 threads hold 17 packs each.
+    // 131071 in 165, 183 where 1024 threads hold 17 packs each; their loss alone in 76 with 512 threads, 88 with 1024, their gradient
+    // alone in 106 with 1024, 117 with 512.
     constexpr int W = 16 / (int)sizeof(T);   // actions of a pack
     const int packs = (q.V + W - 1) / W + 1;   // one more where a row begins inside a pack
     if (q.V <= 16 && q.K <= 16) launch_group<T, 4, 4, MODE>(q, c, st);
@@ -212,7 +215,7 @@ template <typename T, int MODE> static void launch_distill(const DistillArgs &q,
     else if (packs <= 256 * 8) launch_row<T, 256, 8, MODE>(q, c, st);
     else if (packs <= 512 * 8) launch_row<T, 256, 16, MODE>(q, c, st);
     else if (packs <= 8192) launch_row<T, 512, 0, MODE>(q, c, st);
-    else launch_row<T, 1024, 0, MODE>(q, c, st);
+    else launch_row<T, MODE == 0 ? 512 : 1024, 0, MODE>(q, c, st);
 }
 
 template <int MODE> static int run_distill(const mz_distill *a, void *stream, const char *fn)

@@ -123,8 +123,8 @@ constexpr int REC_THREADS = 512;   // of a block: strands of 32 or 64 lanes alon
 // positions in registers; the block's strands follow each other in time and exchange their maps through LDS,
 // one barrier per round of strands, while the next round's loads are on their way.
 // Bound by HBM: 8 x 4096 x 2048 bfloat16 in 102 us (403 MB, 3.95 TB/s where a copy reaches 5.1), 4 x 8192 x 4096 in 195 us
-// forward (4.1 TB/s) and 339 us backward (five tensors, 4.0 TB/s), 32 x 2048 x 4096 in 330 us (4.9 TB/s).  256 tiles are one
-// block of eight waves a compute unit; twice the waves, or twice the positions ahead, change nothing.
+// (4.1 TB/s), 32 x 2048 x 4096 in 330 us (4.9 TB/s).  256 tiles are one block of eight waves a compute unit; twice the waves,
+// or twice the positions ahead, change nothing.
 template <typename T, int VEC, int LANES, int L, bool BWD>
 __global__ __launch_bounds__(REC_THREADS) void k_recurrence_channels(RecurrenceArgs q)
 {
@@ -188,8 +188,8 @@ __global__ __launch_bounds__(REC_THREADS) void k_recurrence_channels(RecurrenceA
 }
 
 // Long records of few channels: a block for every tile would leave compute units idle, so the axis is cut into links of
-// 256 positions (128 in float64) and every link of a tile is a block of its own, with its inputs in registers from the first read to
-// the output.  A link hands two things on through memory: its map, as soon as it has it, and the state behind it, once it
+// 256 positions (128 backward or in float64) and every link of a tile is a block of its own, with its inputs
+// in registers from the first read to the output.  A link hands two things on through memory: its map, as soon as it has it, and the state behind it, once it
 // knows the state in front.  To learn that, it looks back over its predecessors: past those that have only a map yet, to one
 // whose state is known, and folds the maps in between from there on - the same operations in the same order however far it
 // had to look, so results do not depend on timing.
@@ -198,9 +198,11 @@ __global__ __launch_bounds__(REC_THREADS) void k_recurrence_channels(RecurrenceA
 // and that wait for earlier ones in turn: every wait ends.
 // 50000 x 1000 float32 in 140 us (600 MB, 4.3 TB/s) and 5 us for the granules; reading the inputs once for the maps and once for
 // the outputs instead took 211 us, links of half the positions 150, asking four predecessors at once 142 (registers spill).
-constexpr int CHAIN_WAVES = 16, CHAIN_BACK = 16;
+// The gradients of 4 x 8192 x 4096 bfloat16 in 294 us (five tensors, 4.6 TB/s) and 7 for the granules.
+constexpr int CHAIN_BACK = 16;
 constexpr int CHAIN_LENGTH(int size) { return size == 8 ? 8 : 16; }   // positions of a wave; float64 takes twice the registers
-constexpr int CHAIN_ROWS(int size) { return CHAIN_LENGTH(size) * CHAIN_WAVES; }
+constexpr int CHAIN_WAVES(int size, bool backward) { return backward && size != 8 ? 8 : 16; }   // backward: a third tensor in registers
+constexpr int CHAIN_ROWS(int size, bool backward) { return CHAIN_LENGTH(size) * CHAIN_WAVES(size, backward); }
 
 template <typename A> __device__ __forceinline__ void granule_put(unsigned long long *to, A v)
 {
@@ -230,14 +232,14 @@ __global__ void k_zero_granules(unsigned long long *p, long long n)
 }
 
 template <typename T, int VEC, bool BWD>
-__global__ __launch_bounds__(64 * CHAIN_WAVES) void k_recurrence_chain(RecurrenceArgs q)
+__global__ __launch_bounds__(64 * CHAIN_WAVES(sizeof(T), BWD)) void k_recurrence_chain(RecurrenceArgs q)
 {
     using A = acc_t<T>;
     using P = Pack<T, VEC>;
-    constexpr int L = CHAIN_LENGTH(sizeof(T)), ROWS = CHAIN_ROWS(sizeof(T)), W = sizeof(A) / 4;
+    constexpr int L = CHAIN_LENGTH(sizeof(T)), WAVES = CHAIN_WAVES(sizeof(T), BWD), ROWS = CHAIN_ROWS(sizeof(T), BWD), W = sizeof(A) / 4;
     struct Map { A a[VEC], x[VEC]; };
     struct State { A h[VEC]; };
-    __shared__ Map run[CHAIN_WAVES][64], back[CHAIN_BACK][64];
+    __shared__ Map run[WAVES][64], back[CHAIN_BACK][64];
     __shared__ State front[64];
     __shared__ unsigned ticket;
     if (threadIdx.x == 0) ticket = atomicAdd((unsigned *)q.granules, 1u);
@@ -263,7 +265,7 @@ __global__ __launch_bounds__(64 * CHAIN_WAVES) void k_recurrence_chain(Recurrenc
     if (v == 0) {
         // granules of a channel and link: map (a, x), then the state behind it
         auto place = [&](int l, int j) { return q.granules + 8 + (((long long)l * q.B * q.D + row + j) * 3) * W; };
-        for (int i = 1; i < CHAIN_WAVES; i++) {
+        for (int i = 1; i < WAVES; i++) {
             const Map o = run[i][c];
 #pragma unroll
             for (int j = 0; j < VEC; j++) m.x[j] = fma_acc(o.a[j], m.x[j], o.x[j]), m.a[j] *= o.a[j];

@@ -140,8 +140,8 @@ def _recurrence_call(what, gate, x, state, reverse, out, last=None, y=None, out_
     space, need = None, 0
     if T > 256:   # shorter records need none
         size = C.c_int64()
-        _check(lib().mz_linear_recurrence_workspace(_engine.PACK_RECURRENCE(*args, 0, 0), int(y is not None or grad_last is not None),
-                                                    C.byref(size)))
+        _check(lib().mz_linear_recurrence_workspace(_engine.PACK_RECURRENCE(*args, 0, 0),
+                                                    int(what == 'mz_linear_recurrence_backward'), C.byref(size)))
         need = size.value
         space = torch.empty(need, dtype=torch.uint8, device=x.device) if need else None
     _engine.call_operator(what, x.get_device(), _engine.PACK_RECURRENCE(*args, _at(space), need))
