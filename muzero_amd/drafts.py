@@ -78,7 +78,8 @@ def verify_by_search(mcts, network, observations, legal_actions, to_play, tokens
 
     observations [B, K + 1, ...], legal_actions [B, K + 1, A], to_play [B, K + 1]: the position in front of every drafted move
     and the one behind the last (behind a game's own length: any position).  tokens [B, K] device int32 / int64, draft
-    [B, K, A] device float64 or None.  At `temperature` 0 the searched policy is its best move alone.
+    [B, K, A] device float64 or None.  `temperature` as for `search_batch`: at 0 a PUCT search's policy is its most visited move
+    (shared where several tie), a Gumbel search has none.
     Returns (accepted, moves, root values [B, K + 1])."""
     B, K = tokens.shape
     observations = observations if torch.is_tensor(observations) else np.asarray(observations)

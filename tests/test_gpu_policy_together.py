@@ -64,3 +64,40 @@ def test_self_play_returns_distillation_and_drafts():
     n, want = plain_rule(tokens, draft, target, ua, us, None)
     np.testing.assert_array_equal(accepted.cpu().numpy(), n)
     np.testing.assert_array_equal(moves.cpu().numpy(), want)
+
+
+def test_a_captured_training_step():
+    """Forward and backward of the recurrence and the distillation in one graph, replayed over new inputs; the leaves belong to
+    the capture alone (an eager graph of the same leaves must not live while a backward pass is captured)."""
+    from muzero_amd.targets import linear_recurrence
+    from muzero_amd.trainer import distillation_loss
+    gen = torch.Generator().manual_seed(0)
+    new = lambda *s: torch.randn(s, generator=gen).cuda()  # noqa: E731
+    T, V = 900, 70                                          # a chain of links forward and backward, rows of two packs
+    gate, x, dy = torch.sigmoid(new(1, T, V)), new(1, T, V), new(1, T, V)
+    index = torch.randint(0, V, (T, 3), generator=gen).cuda()
+    teacher, up = new(T, 3), torch.rand(T, generator=gen).cuda()
+
+    def step(gate, x):
+        y, _ = linear_recurrence(gate, x)
+        loss = distillation_loss(y[0], index, teacher)
+        return (loss,) + torch.autograd.grad(loss, (gate, x), up)
+
+    leaves = lambda: (gate.clone().requires_grad_(), x.clone().requires_grad_())  # noqa: E731
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(*leaves())
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    g, z = leaves()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step(g, z)
+    for i in range(4):
+        with torch.no_grad():
+            z.copy_(x * (1 + i))
+        graph.replay()
+        want = step(gate.clone().requires_grad_(), (x * (1 + i)).requires_grad_())
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(out, want))
