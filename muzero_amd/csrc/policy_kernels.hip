@@ -26,8 +26,11 @@ static size_t size_of(int type) { return type == MZ_F64 ? 8 : type == MZ_F32 ? 4
 //   three links (1 x 600 x 512) 11.2 against 10.5, their gradients 15.3 against 17.6.  Gradients, with five tensors on their
 //   way, gain up to REC_FEW_TILES_BACKWARD tiles: 4 x 8192 x 4096 (256 tiles) 301 against 334, 8 x 2048 x 2500 (320) 114
 //   against 159.
+// - Fewer than REC_FEW_ROWS rows of REC_LEAST_ROW_LINKS links or more are cut into links: 1 x 65536 float32 7.9 against 18.1 us (the
+//   granules' 2 us included), 64 x 32768 13.1 against 13.3, its gradients 15.7 against 18.5; 200 x 32768 23.7 against 16.7.
 constexpr int REC_LENGTH = 8;
 constexpr long long REC_MANY_TILES = 512, REC_FEW_TILES = 256, REC_FEW_TILES_BACKWARD = 512, REC_LEAST_LINKS = 3;
+constexpr long long REC_FEW_ROWS = 128, REC_LEAST_ROW_LINKS = 3;
 
 // How a recurrence is run: chosen by sizes, strides and alignment alone, for the workspace query and the call alike.
 struct RecurrencePlan {
@@ -48,7 +51,11 @@ static RecurrencePlan plan_recurrence(const mz_recurrence *a, bool backward)
         low |= (uint64_t)(uintptr_t)t->p | (uint64_t)t->stride_b * size | (uint64_t)t->stride_t * size;
     }
     if (a->D == 1) p.channels = false;
-    if (!p.channels) return p;
+    if (!p.channels) {
+        const long long links = (a->T + ROW_LINK - 1) / ROW_LINK;
+        if ((long long)a->B * a->D < REC_FEW_ROWS && links >= REC_LEAST_ROW_LINKS && links < INT32_MAX / REC_FEW_ROWS) p.links = (int)links;
+        return p;
+    }
     auto fits = [&](int n) { return a->D % n == 0 && low % (uint64_t)(n * size) == 0; };
     // a step, or a few: the block of strands would stand idle (64 x 4 x 4096 bfloat16 4.1 against 5.8 us, 8 positions 4.8 against
     // 6.4, 16 positions 7.2 against 6.6)
@@ -78,11 +85,16 @@ static size_t granule_count(const mz_recurrence *a, const RecurrencePlan &p)
     return p.links ? 8 + (size_t)p.links * a->B * a->D * 3 * (a->type == MZ_F64 ? 2 : 1) : 0;
 }
 
-template <typename T, int VEC, bool BWD> static void launch_chain(const RecurrenceArgs &q, hipStream_t st)
+template <typename T> static void zero_granules(const RecurrenceArgs &q, hipStream_t st)
 {
     const long long granules = 8 + (long long)q.links * q.B * q.D * 3 * (long long)(sizeof(acc_t<T>) / 4);
     const unsigned blocks = (unsigned)std::min<long long>((granules + 255) / 256, 2048);
     hipLaunchKernelGGL(k_zero_granules, dim3(blocks), dim3(256), 0, st, q.granules, granules);
+}
+
+template <typename T, int VEC, bool BWD> static void launch_chain(const RecurrenceArgs &q, hipStream_t st)
+{
+    zero_granules<T>(q, st);
     const long long tiles = (long long)q.B * ((q.D + 64 * VEC - 1) / (64 * VEC));
     hipLaunchKernelGGL((k_recurrence_chain<T, VEC, BWD>), dim3((unsigned)(tiles * q.links)), dim3(64 * CHAIN_WAVES(sizeof(T), BWD)), 0, st, q);
 }
@@ -111,7 +123,10 @@ template <typename T, int E, bool BWD> static void launch_rows(const RecurrenceA
 template <typename T, bool BWD> static void launch_recurrence(const RecurrencePlan &p, const RecurrenceArgs &q, hipStream_t st)
 {
     constexpr int W = 16 / (int)sizeof(T);
-    if (!p.channels) {
+    if (!p.channels && p.links) {
+        zero_granules<T>(q, st);
+        hipLaunchKernelGGL((k_recurrence_row_chain<T, BWD>), dim3((unsigned)((long long)q.B * q.D * q.links)), dim3(1024), 0, st, q);
+    } else if (!p.channels) {
         // positions a thread: 4000 rows of 500 float32 in 7.5 us with 8, 9.9 with 2; of 250 in 6.3 and 6.5, of 60 in 6.0 and 4.8
         if (q.T > 256) launch_rows<T, 8, BWD>(q, st);
         else launch_rows<T, 2, BWD>(q, st);

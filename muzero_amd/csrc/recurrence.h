@@ -384,7 +384,7 @@ template <typename T, int E> struct Stretch {
 
 // Any strides, one row (b, d) per block: every thread walks E consecutive positions, the maps are composed across the wave
 // by shuffles and across the waves through LDS.  1000 rows of 4097 float32 in 11.7 us forward and 20.6 backward (49 and 82 MB,
-// 4.2 and 4.0 TB/s); few very long rows keep few compute units busy (one block walks 8192 float32 positions in about 2.5 us).
+// 4.2 and 4.0 TB/s); a block walks 8192 float32 positions of a long row in about 2.3 us.
 template <typename T, int E, bool BWD>
 __global__ __launch_bounds__(1024) void k_recurrence_rows(RecurrenceArgs q)
 {
@@ -443,6 +443,98 @@ __global__ __launch_bounds__(1024) void k_recurrence_rows(RecurrenceArgs q)
     if (q.last && threadIdx.x == 0) {
         if (BWD) carry *= widen(*at<T>(q.a, b, q.T - 1, d));
         ((A *)q.last)[blockIdx.x] = carry;
+    }
+}
+
+// A few long rows: links of ROW_LINK positions of one row, a block each, handed on as in k_recurrence_chain; a wave looks back
+// over 64 predecessors at once, a lane each.  One row of 4 000 000 float32 in 32 us (48 MB; 1118 us walked by one block).
+constexpr int ROW_STRETCH = 8, ROW_LINK = 1024 * ROW_STRETCH;
+
+template <typename T, bool BWD>
+__global__ __launch_bounds__(1024) void k_recurrence_row_chain(RecurrenceArgs q)
+{
+    using A = acc_t<T>;
+    constexpr int E = ROW_STRETCH, W = sizeof(A) / 4, WAVES = 16;
+    __shared__ A run_a[WAVES], run_x[WAVES], front;
+    __shared__ unsigned ticket;
+    if (threadIdx.x == 0) ticket = atomicAdd((unsigned *)q.granules, 1u);
+    __syncthreads();
+    const int rows = q.B * q.D, link = (int)(ticket / (unsigned)rows), row = (int)(ticket % (unsigned)rows);
+    const int b = row / q.D, d = row % q.D, lane = threadIdx.x % 64, w = threadIdx.x / 64;
+    const bool want_da = BWD && q.da.p;
+    const long long s0 = (long long)link * ROW_LINK + threadIdx.x * E;
+    Stretch<T, E> a, x, y;
+    x.load(q.x, at<T>(q.x, b, 0, d), s0, q.T, T(0.0f));
+    if (!BWD) a.load(q.a, at<T>(q.a, b, 0, d), s0, q.T, T(1.0f));
+    else {
+        a.load(q.a, at<T>(q.a, b, 0, d), s0 - 1, q.T, T(1.0f));
+        if (want_da) y.load(q.y, at<T>(q.y, b, 0, d), s0 + 1, q.T, T(0.0f));
+        if (s0 + E > q.T)
+#pragma unroll
+            for (int i = 0; i < E; i++) if (s0 + i >= q.T) a.v[i] = T(1.0f);
+    }
+    A ra = A(1), rx = A(0);
+#pragma unroll
+    for (int i = 0; i < E; i++) rx = fma_acc(widen(a.v[i]), rx, widen(x.v[i])), ra *= widen(a.v[i]);
+#pragma unroll
+    for (int k = 1; k < 64; k *= 2) {
+        const A pa = __shfl_up(ra, k), px = __shfl_up(rx, k);
+        if (lane >= k) rx = fma_acc(ra, px, rx), ra *= pa;
+    }
+    if (lane == 63) run_a[w] = ra, run_x[w] = rx;
+    A ea = __shfl_up(ra, 1), ex = __shfl_up(rx, 1);
+    if (lane == 0) ea = A(1), ex = A(0);
+    lds_fence_barrier();
+    if (w == 0) {
+        auto place = [&](int l) { return q.granules + 8 + (((long long)l * rows + row) * 3) * W; };
+        A ma = run_a[0], mx = run_x[0];
+        for (int i = 1; i < WAVES; i++) mx = fma_acc(run_a[i], mx, run_x[i]), ma *= run_a[i];
+        A h;
+        if (link == 0) h = state_at<A>(q.first, row);
+        else {
+            if (lane == 0) granule_put(place(link), ma), granule_put(place(link) + W, mx);
+            A oa, ox, oh;
+            int known_at;
+            while (true) {
+                const bool there = lane < link;   // predecessor link - 1 - lane; link 0 hands on its state alone
+                const unsigned long long *p = place(there ? link - 1 - lane : 0);
+                const bool known = granule_get(p + 2 * W, oh), has_a = granule_get(p, oa), has_x = granule_get(p + W, ox);
+                const unsigned long long states = __ballot(there && known), maps = __ballot(there && has_a && has_x);
+                if (states) {
+                    known_at = __ffsll((long long)states) - 1;
+                    const unsigned long long nearer = (1ull << known_at) - 1;
+                    if ((maps & nearer) == nearer) break;
+                }
+                __builtin_amdgcn_s_sleep(1);
+            }
+            known_at = __builtin_amdgcn_readfirstlane(known_at);
+            h = lane_read(oh, known_at);
+            for (int i = known_at - 1; i >= 0; i--) h = fma_acc(lane_read(oa, i), h, lane_read(ox, i));
+        }
+        const A behind = fma_acc(ma, h, mx);
+        if (lane == 0) {
+            if (link + 1 < q.links) granule_put(place(link) + 2 * W, behind);
+            front = h;
+            if (q.last && link + 1 == q.links) ((A *)q.last)[row] = BWD ? behind * widen(*at<T>(q.a, b, q.T - 1, d)) : behind;
+        }
+    }
+    lds_fence_barrier();
+    if (s0 >= q.T) return;
+    A h = front;
+    for (int i = 0; i < w; i++) h = fma_acc(run_a[i], h, run_x[i]);
+    h = fma_acc(ea, h, ex);
+    Stretch<T, E> o, da;
+#pragma unroll
+    for (int i = 0; i < E; i++) {
+        h = fma_acc(widen(a.v[i]), h, widen(x.v[i]));
+        o.v[i] = narrow<T>(h);
+        if constexpr (BWD) {
+            if (want_da) da.v[i] = narrow<T>(h * (s0 + i + 1 == q.T ? state_at<A>(q.state0, row) : widen(y.v[i])));
+        }
+    }
+    o.store(q.out, (T *)at<T>(q.out, b, 0, d), s0, q.T);
+    if constexpr (BWD) {
+        if (want_da) da.store(q.da, (T *)at<T>(q.da, b, 0, d), s0, q.T);
     }
 }
 

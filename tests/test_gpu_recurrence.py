@@ -293,6 +293,34 @@ def test_chains_of_links(shape, dtype):
         assert all(torch.equal(o, y) and torch.equal(l, last) for o, l in outs)
 
 
+@pytest.mark.parametrize('dtype', TYPES)
+def test_long_rows(dtype):
+    """Rows of one channel cut into links, and channels contiguous in time: right, and the same bits every time."""
+    from muzero_amd.targets import linear_recurrence
+    for B, T, D in ((2, 16385, 1), (1, 24577, 3)):
+        a, x, s = inputs(B, T, D, dtype, seed=T)
+        dy = torch.randn(B, T, D, generator=torch.Generator().manual_seed(1)).to(dtype).cuda()
+        rows = lambda t: t.transpose(1, 2).contiguous().transpose(1, 2).requires_grad_()  # noqa: E731
+        for reverse in (False, True):
+            y_ref, last_ref = loop(a, x, s, reverse)
+            z, zl = loop(a.abs(), x.abs(), s.abs(), reverse)
+            dx_ref, da_ref, ds_ref = loop_backward(a, y_ref, s, dy, s, reverse)
+            zx, zda, zs = loop_backward(a.abs(), z, s.abs(), dy.abs(), s.abs(), reverse)
+            first = None
+            for _ in range(3):
+                leaves = (rows(a), rows(x), s.clone().requires_grad_())
+                y, last = linear_recurrence(*leaves, reverse=reverse)
+                out = (y, last) + torch.autograd.grad((y, last), leaves, (rows(dy).detach(), s))
+                first = first or out
+                assert all(torch.equal(p, q) for p, q in zip(out, first))
+            close(first[0], y_ref, z, T, dtype)
+            close(first[1], last_ref, zl, T, dtype)
+            close(first[3], dx_ref, zx, T, dtype)
+            close(first[4], ds_ref, zs, T + 1, dtype)
+            half = torch.finfo(dtype).eps / 2
+            close(first[2], da_ref, 2 * zda, T, dtype, extra=half * zda + (2.0 ** -25 * zx if dtype == torch.float16 else 0.0))
+
+
 def test_offsets_beyond_32_bits():
     """Sequences, positions and channels whose distance in memory passes 2^31 elements."""
     from muzero_amd.targets import linear_recurrence
