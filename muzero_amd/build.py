@@ -1,14 +1,18 @@
-"""Builds the HIP engine in-tree: muzero_amd/libmuzero_amd.so (gfx950 only)."""
+"""Builds the HIP engine in-tree: muzero_amd/libmuzero_amd.so (gfx950 only), and the host-side binding of the tensor operators
+to torch, muzero_amd/_torch_calls.so."""
 from __future__ import annotations
 
 import os
 import subprocess
+import sysconfig
 from concurrent.futures import ThreadPoolExecutor
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, 'csrc')
 LIB = os.path.join(HERE, 'libmuzero_amd.so')
 OBJ_DIR = os.path.join(HERE, 'build')
+TORCH_LIB = os.path.join(HERE, '_torch_calls.so')
+TORCH_SOURCE = os.path.join(CSRC, 'torch_calls.cpp')
 # translation units: the C ABI with the tree / fused-network kernels, the matrix-core kernels, and the tensor operators
 SOURCES = ['engine.hip', 'mfma_kernels.hip', 'chain_kernels.hip', 'cached_kernels_a.hip', 'cached_kernels_b.hip',
            'cached_kernels_c.hip', 'policy_kernels.hip']
@@ -75,9 +79,34 @@ def _stale(src: str, obj: str) -> bool:
     return any(os.path.getmtime(os.path.join(CSRC, f)) > t for f in deps)
 
 
+def build_torch_calls(force: bool = False) -> str:
+    """Host code only (the host compiler, torch's headers and libraries; no GPU headers)."""
+    deps = [TORCH_SOURCE, os.path.join(HERE, '..', 'include', 'muzero_amd.h')]
+    if force or not os.path.exists(TORCH_LIB) or any(os.path.getmtime(f) > os.path.getmtime(TORCH_LIB) for f in deps):
+        import torch
+        root = os.path.dirname(torch.__file__)
+        include = [os.path.join(root, 'include'), os.path.join(root, 'include', 'torch', 'csrc', 'api', 'include'),
+                   sysconfig.get_paths()['include']]
+        libs = os.path.join(root, 'lib')
+        subprocess.check_call([os.environ.get('CXX', 'g++'), '-O2', '-std=c++17', '-fPIC', '-shared', '-DTORCH_EXTENSION_NAME=_torch_calls',
+                               '-DTORCH_API_INCLUDE_EXTENSION_H', f'-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}',
+                               *[f'-I{i}' for i in include], TORCH_SOURCE, '-o', TORCH_LIB, f'-L{libs}', f'-Wl,-rpath,{libs}', '-lc10',
+                               '-ltorch_cpu', '-ltorch_python'])
+    return TORCH_LIB
+
+
 def build(force: bool = False, defines=(), lib: str = LIB) -> str:
     """Compiles the translation units that changed (all of them with `force`), in parallel, and links the shared
     library.  `defines`: extra -D flags (the diagnostic build with phase stamps uses MZ_STAMPS and another `lib`)."""
+    with ThreadPoolExecutor(1) as beside:
+        binding = beside.submit(build_torch_calls, force) if lib == LIB else None
+        _build_library(force, defines, lib)
+        if binding is not None:
+            binding.result()
+    return lib
+
+
+def _build_library(force, defines, lib) -> None:
     if force or needs_build(lib):
         hipcc = os.environ.get('HIPCC', '/opt/rocm/bin/hipcc')
         os.makedirs(OBJ_DIR, exist_ok=True)
@@ -92,7 +121,6 @@ def build(force: bool = False, defines=(), lib: str = LIB) -> str:
         with ThreadPoolExecutor(max(len(todo), 1)) as pool:
             list(pool.map(compile_one, todo))
         subprocess.check_call([hipcc, '--offload-arch=gfx950', '-shared', '-fPIC', *objs, '-o', lib])
-    return lib
 
 
 if __name__ == '__main__':

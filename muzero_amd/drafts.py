@@ -50,23 +50,7 @@ def verify_drafts(tokens: torch.Tensor, draft: Optional[torch.Tensor], target: t
         raise ValueError('verify_drafts: u_accept [B, K] and u_sample [B] must be float64')
     if lengths is not None and (tuple(lengths.shape) != (B,) or lengths.dtype != torch.int32):
         raise ValueError('verify_drafts: lengths must be int32 [B]')
-    accepted = u_sample.new_empty((B,), dtype=torch.int32)
-    out = tokens.new_empty((B, K + 1))
-    if B == 0:
-        return accepted, out
-    if target.stride(2) != 1 and V > 1:
-        target = target.contiguous()
-    if draft is not None and draft.stride(2) != 1 and V > 1:
-        draft = draft.contiguous()
-    tokens, u_accept, u_sample = tokens.contiguous(), u_accept.contiguous(), u_sample.contiguous()
-    lengths = None if lengths is None else lengths.contiguous()
-    p = lambda t: 0 if t is None else t.data_ptr()  # noqa: E731
-    sd = (0, 0) if draft is None else draft.stride()[:2]
-    args = _engine.PACK_VERIFY(_engine.ELEMENT_TYPES[target.dtype], int(tokens.dtype == torch.int64), B, K, V, 0, p(tokens), p(draft),
-                               *sd, p(target), target.stride(0), target.stride(1), p(u_accept), p(u_sample), p(lengths),
-                               p(accepted), p(out))
-    _engine.call_operator('mz_verify_drafts', where, args)
-    return accepted, out
+    return _engine.torch_calls().verify_drafts(tokens, draft, target, u_accept, u_sample, lengths, _engine.raw_stream(where))
 
 
 def verify_by_search(mcts, network, observations, legal_actions, to_play, tokens: torch.Tensor, draft: Optional[torch.Tensor],

@@ -7,8 +7,8 @@ library is missing, importing this module's engine raises.
 from __future__ import annotations
 
 import ctypes as C
+import importlib.util
 import os
-import struct
 
 import numpy as np
 import torch
@@ -81,11 +81,6 @@ class MzVerify(C.Structure):
 
 
 ENV_TICTACTOE, ENV_CARTPOLE = 1, 2
-# The same layouts as flat packers: the tensor operators' calls are short enough for the fields of a ctypes structure, set one
-# by one, to cost more than the launch.
-PACK_RECURRENCE = struct.Struct('@4iq20q6q').pack
-PACK_DISTILL = struct.Struct('@6if10q').pack
-PACK_VERIFY = struct.Struct('@6i12q').pack
 # element types of the tensor operators (MZ_F32 ...)
 ELEMENT_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2, torch.float64: 3}
 
@@ -235,22 +230,30 @@ def _stream():
     return C.c_void_p(torch.cuda.current_stream().cuda_stream)
 
 
-_calls = {}
+_torch_calls = None
 
 
-def call_operator(what: str, device: int, args: bytes) -> None:
-    """Calls a tensor operator's entry point with a packed argument struct, on the current stream of the tensors' device (an
-    index, which need not be the current one)."""
-    fn = _calls.get(what)
-    if fn is None:
-        fn = _calls[what] = getattr(lib(), what)
-    if device == torch._C._cuda_getDevice():
-        rc = fn(args, torch._C._cuda_getCurrentRawStream(device))
-    else:
-        with torch.cuda.device(device):
-            rc = fn(args, torch._C._cuda_getCurrentRawStream(device))
-    if rc:
-        _check(rc, what)
+def torch_calls():
+    """The native calls of the tensor operators (csrc/torch_calls.cpp), bound to the loaded library; raises if not built."""
+    global _torch_calls
+    if _torch_calls is None:
+        L = lib()
+        path = os.path.join(_HERE, '_torch_calls.so')
+        if not os.path.exists(path):
+            raise EngineError(f'{path} is missing: build it with `python -m muzero_amd.build`. There is no CPU fallback.')
+        spec = importlib.util.spec_from_file_location('_torch_calls', path)
+        module = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(module)
+        module.bind([C.cast(getattr(L, name), C.c_void_p).value for name in (
+            'mz_linear_recurrence', 'mz_linear_recurrence_backward', 'mz_linear_recurrence_workspace', 'mz_distill_loss', 'mz_distill_grad',
+            'mz_distill_loss_grad', 'mz_verify_drafts', 'mz_last_error')])
+        _torch_calls = module
+    return _torch_calls
+
+
+def raw_stream(device: int) -> int:
+    """The current torch stream of a device, which need not be the current one, as an address."""
+    return torch._C._cuda_getCurrentRawStream(device)
 
 
 class SearchEngine:

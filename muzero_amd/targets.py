@@ -104,97 +104,6 @@ def scalar_to_support(x: torch.Tensor, support_limit: int) -> torch.Tensor:
 _STATE_TYPE = {torch.float64: torch.float64}
 
 
-def _lined_up(t: torch.Tensor, channels: bool) -> torch.Tensor:
-    """`t` itself where the kernels read its layout well: channels contiguous, or (one channel, or time contiguous) any."""
-    return t.contiguous() if channels and t.stride(2) != 1 else t
-
-
-def _like(x: torch.Tensor, channels: bool) -> torch.Tensor:
-    y = torch.empty_like(x)
-    return torch.empty(x.shape, dtype=x.dtype, device=x.device) if channels and y.stride(2) != 1 else y
-
-
-def _view(t):
-    return (0, 0, 0, 0) if t is None else (t.data_ptr(), *t.stride())
-
-
-def _at(t):
-    return 0 if t is None else t.data_ptr()
-
-
-def _recurrence_call(what, gate, x, state, reverse, out, last=None, y=None, out_gate=None, grad_last=None, out_state=None):
-    B, T, D = x.shape
-    if D == 1 and B > 1 and x.stride(0) == 1 and (T == 1 or x.stride(1) != 1):
-        # one channel, time-major (or a single position): the sequences are the channels of one
-        turned = [None if v is None else v.transpose(0, 2) for v in (gate, x, out, y, out_gate)]
-        if all(v is None or v.stride(2) == 1 for v in turned):
-            gate, x, out, y, out_gate = turned
-            B, D = 1, B
-    if x.is_contiguous() and gate.is_contiguous() and out.is_contiguous() and (y is None or y.is_contiguous() and out_gate.is_contiguous()):
-        n = T * D
-        args = (_engine.ELEMENT_TYPES[x.dtype], B, D, reverse, T, gate.data_ptr(), n, D, 1, x.data_ptr(), n, D, 1,
-                out.data_ptr(), n, D, 1, _at(y), n, D, 1, _at(out_gate), n, D, 1, _at(state), _at(last), _at(grad_last), _at(out_state))
-    else:
-        args = (_engine.ELEMENT_TYPES[x.dtype], B, D, reverse, T, *_view(gate), *_view(x), *_view(out), *_view(y), *_view(out_gate),
-                _at(state), _at(last), _at(grad_last), _at(out_state))
-    space, need = None, 0
-    if T > 256:   # shorter records need none
-        size = C.c_int64()
-        _check(lib().mz_linear_recurrence_workspace(_engine.PACK_RECURRENCE(*args, 0, 0),
-                                                    int(what == 'mz_linear_recurrence_backward'), C.byref(size)))
-        need = size.value
-        space = torch.empty(need, dtype=torch.uint8, device=x.device) if need else None
-    _engine.call_operator(what, x.get_device(), _engine.PACK_RECURRENCE(*args, _at(space), need))
-
-
-def _recurrence_forward(gate, x, state, reverse):
-    B, T, D = x.shape
-    wide = _STATE_TYPE.get(x.dtype, torch.float32)
-    if x.numel() == 0:
-        return torch.empty_like(x), torch.zeros((B, D), dtype=wide, device=x.device) if state is None else state.clone()
-    channels = D > 1 and (x.stride(2) == 1 or x.stride(1) != 1)
-    gate, x = _lined_up(gate, channels), _lined_up(x, channels)
-    y, last = _like(x, channels), x.new_empty((B, D), dtype=wide)
-    _recurrence_call('mz_linear_recurrence', gate, x, state, reverse, y, last)
-    return y, last
-
-
-class _LinearRecurrence(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, gate, x, state, reverse):
-        y, last = _recurrence_forward(gate, x, state, reverse)
-        ctx.reverse = reverse
-        ctx.set_materialize_grads(False)
-        ctx.save_for_backward(gate, y if ctx.needs_input_grad[0] else None, state)
-        return y, last
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, dy, dlast):
-        if dy is None and dlast is None:
-            return None, None, None, None
-        gate, y, state = ctx.saved_tensors
-        want_gate, want_x, want_state, _ = ctx.needs_input_grad
-        if dy is None:
-            dy = torch.zeros(gate.shape, dtype=gate.dtype, device=gate.device)
-        if dlast is not None:
-            dlast = dlast.contiguous()
-        B, T, D = dy.shape
-        dstate = dy.new_empty((B, D), dtype=_STATE_TYPE.get(dy.dtype, torch.float32)) if want_state else None
-        if dy.numel() == 0:
-            return (torch.empty_like(dy) if want_gate else None, torch.empty_like(dy) if want_x else None,
-                    None if not want_state else torch.zeros_like(dstate) if dlast is None else dlast.clone(), None)
-        channels = D > 1 and (dy.stride(2) == 1 or dy.stride(1) != 1)
-        gate, dy = _lined_up(gate, channels), _lined_up(dy, channels)
-        dx, dgate = _like(dy, channels), None
-        if want_gate:
-            y, dgate = _lined_up(y, channels), _like(dy, channels)
-        else:
-            y = None
-        _recurrence_call('mz_linear_recurrence_backward', gate, dy, state, ctx.reverse, dx, None, y, dgate, dlast, dstate)
-        return dgate, dx if want_x else None, dstate, None
-
-
 def linear_recurrence(gate: torch.Tensor, x: torch.Tensor, state: Optional[torch.Tensor] = None, reverse: bool = False):
     """y[:, t] = gate[:, t] * y[:, t-1] + x[:, t] along axis 1 of device tensors [B, T, D] (`reverse`: from the last
     position to the first, the direction of returns), differentiable in gate, x and state.
@@ -214,16 +123,12 @@ def linear_recurrence(gate: torch.Tensor, x: torch.Tensor, state: Optional[torch
         raise ValueError(f'linear_recurrence: gate and x must share a floating type, got {gate.dtype} and {dtype}')
     if gate.get_device() != x.get_device():
         raise ValueError('linear_recurrence: gate and x are on different devices')
-    grads = gate.requires_grad or x.requires_grad
+    where = x.get_device()
     if state is not None:
         wide = _STATE_TYPE.get(dtype, torch.float32)
-        if not torch.is_tensor(state) or state.shape != (shape[0], shape[2]) or state.dtype != wide or state.get_device() != x.get_device():
+        if not torch.is_tensor(state) or state.shape != (shape[0], shape[2]) or state.dtype != wide or state.get_device() != where:
             raise ValueError(f'linear_recurrence: state must be {wide} [{shape[0]}, {shape[2]}] on the device of x')
-        state = state.contiguous()
-        grads = grads or state.requires_grad
-    if grads and torch.is_grad_enabled():
-        return _LinearRecurrence.apply(gate, x, state, bool(reverse))
-    return _recurrence_forward(gate, x, state, bool(reverse))
+    return _engine.torch_calls().linear_recurrence(gate, x, state, bool(reverse), _engine.raw_stream(where))
 
 
 class TrajectoryStore:

@@ -62,63 +62,29 @@ def _refuse(logits, index, teacher, teacher_lse, weight):
     if logits.dim() != 2 or index.dim() != 2 or index.shape[0] != logits.shape[0] or teacher.shape != index.shape:
         raise ValueError(f'distillation: logits [R, V], index and teacher [R, K] expected, got {tuple(logits.shape)}, '
                          f'{tuple(index.shape)}, {tuple(teacher.shape)}')
-    if logits.dtype not in _LOGIT_TYPES or teacher.dtype not in _LOGIT_TYPES or index.dtype not in _INDEX_TYPES:
+    if logits.dtype not in _LOGIT_TYPES or teacher.dtype not in _LOGIT_TYPES or index.dtype not in (torch.int32, torch.int64):
         raise ValueError('distillation: logits and teacher are float32, bfloat16 or float16, index is int32 or int64')
     raise ValueError(f'distillation: teacher_lse and weight must be float32 [{logits.shape[0]}]')
 
 
-_LOGIT_TYPES = {t: k for t, k in _engine.ELEMENT_TYPES.items() if t != torch.float64}
-_INDEX_TYPES = {torch.int32: 0, torch.int64: 1}
+_LOGIT_TYPES = frozenset((torch.float32, torch.bfloat16, torch.float16))
 
 
-def _distill_args(logits, index, teacher, lse, weight):
-    """The tensors a distillation call points to: checked, and contiguous where they have to be."""
+def _check_distillation(logits, index, teacher, lse, weight) -> int:
+    """The stream of a distillation call whose arguments fit."""
     try:
         R, _ = logits.shape
         where = logits.get_device()
         fits = (where >= 0 and index.get_device() == where and teacher.get_device() == where and index.shape[0] == R
                 and len(index.shape) == 2 and teacher.shape == index.shape and logits.dtype in _LOGIT_TYPES
-                and teacher.dtype in _LOGIT_TYPES and index.dtype in _INDEX_TYPES
-                and all(t is None or (t.shape == (R,) and t.dtype == torch.float32 and t.get_device() == where) for t in (lse, weight)))
+                and teacher.dtype in _LOGIT_TYPES and (index.dtype == torch.int64 or index.dtype == torch.int32)
+                and (lse is None or (lse.shape == (R,) and lse.dtype == torch.float32 and lse.get_device() == where))
+                and (weight is None or (weight.shape == (R,) and weight.dtype == torch.float32 and weight.get_device() == where)))
     except (AttributeError, ValueError, TypeError, IndexError):
         fits = False
     if not fits:
         _refuse(logits, index, teacher, lse, weight)
-    if logits.stride(1) != 1 or logits.stride(0) < 0:
-        logits = logits.contiguous()
-    return (logits, index.contiguous(), teacher.contiguous(), None if lse is None else lse.contiguous(),
-            None if weight is None else weight.contiguous())
-
-
-def _distill_call(what, tensors, temperature, grad_loss=0, loss=0, grad=0, stats=0):
-    logits, index, teacher, lse, weight = tensors
-    R, V = logits.shape
-    if R:
-        _engine.call_operator(what, logits.get_device(), _engine.PACK_DISTILL(
-            _LOGIT_TYPES[logits.dtype], _LOGIT_TYPES[teacher.dtype], _INDEX_TYPES[index.dtype], R, V, index.shape[1], temperature,
-            logits.data_ptr(), logits.stride(0), index.data_ptr(), teacher.data_ptr(), 0 if lse is None else lse.data_ptr(),
-            0 if weight is None else weight.data_ptr(), grad_loss, loss, grad, stats))
-
-
-class _Distillation(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, logits, index, teacher, teacher_lse, temperature, weight):
-        tensors = _distill_args(logits, index, teacher, teacher_lse, weight)
-        R = logits.shape[0]
-        loss, stats = logits.new_empty((R,), dtype=torch.float32), logits.new_empty((R, 4), dtype=torch.float32)
-        _distill_call('mz_distill_loss', tensors, temperature, loss=loss.data_ptr(), stats=stats.data_ptr())
-        ctx.save_for_backward(*tensors, stats)
-        ctx.temperature = temperature
-        return loss
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, up):
-        *tensors, stats = ctx.saved_tensors
-        grad = torch.empty(tensors[0].shape, dtype=tensors[0].dtype, device=up.device)
-        up = up.contiguous()
-        _distill_call('mz_distill_grad', tensors, ctx.temperature, up.data_ptr(), 0, grad.data_ptr(), stats.data_ptr())
-        return grad, None, None, None, None, None
+    return _engine.raw_stream(where)
 
 
 def distillation_loss(logits: torch.Tensor, index: torch.Tensor, teacher: torch.Tensor, teacher_lse: Optional[torch.Tensor] = None,
@@ -132,18 +98,16 @@ def distillation_loss(logits: torch.Tensor, index: torch.Tensor, teacher: torch.
     logits / temperature over all actions, keeps its remaining mass as one more class; without it p is renormalised over the
     entries.  weight float32 [R]: rows of weight 0 and rows without entries have loss and gradient 0 whatever they hold.
     A row whose logits are all -inf, or that holds NaN, gives NaN; an action of probability 0 that the teacher names gives inf."""
-    return _Distillation.apply(logits, index, teacher, teacher_lse, float(temperature), weight)
+    stream = _check_distillation(logits, index, teacher, teacher_lse, weight)
+    return _engine.torch_calls().distillation_loss(logits, index, teacher, teacher_lse, weight, float(temperature), stream)
 
 
 def distillation_loss_grad(logits: torch.Tensor, index: torch.Tensor, teacher: torch.Tensor, teacher_lse: Optional[torch.Tensor] = None,
                            temperature: float = 1.0, weight: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
     """`distillation_loss` and its gradient d loss[r] / d logits (type and shape of logits) in one pass that reads the logits
     once; scale rows through `weight`.  For training loops that hand the gradient to `logits.backward(grad)` themselves."""
-    tensors = _distill_args(logits, index, teacher, teacher_lse, weight)
-    loss = logits.new_empty((logits.shape[0],), dtype=torch.float32)
-    grad = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
-    _distill_call('mz_distill_loss_grad', tensors, float(temperature), 0, loss.data_ptr(), grad.data_ptr())
-    return loss, grad
+    stream = _check_distillation(logits, index, teacher, teacher_lse, weight)
+    return _engine.torch_calls().distillation_loss_grad(logits, index, teacher, teacher_lse, weight, float(temperature), stream)
 
 
 def build_optimizer(network: nn.Module, config) -> torch.optim.Optimizer:
