@@ -20,12 +20,14 @@ struct VerifyArgs {
     int B, K, V, token64;
 };
 
-// Entries that are no probability (negative, NaN, infinite) count as zero.
+// Entries that are no probability (negative, NaN, infinite) count as zero; looked at in the type's own precision, which costs a
+// third of the same in float64.
 template <typename T> __device__ __forceinline__ double mass_of(T v)
 {
-    const double d = (double)v;
-    return d > 0 && d < HUGE_VAL ? d : 0.0;
+    const float f = (float)v;
+    return (double)fmaxf(f < HUGE_VALF ? f : 0.0f, 0.0f);
 }
+template <> __device__ __forceinline__ double mass_of(double d) { return d > 0 && d < HUGE_VAL ? d : 0.0; }
 
 __device__ __forceinline__ long long drafted(const VerifyArgs &q, long long i)
 {
@@ -66,8 +68,8 @@ template <typename T> struct Left {
     __device__ __forceinline__ bool whole() const { return !d && only < 0; }
     __device__ __forceinline__ double of(T pj, T dj, int j) const
     {
-        const double v = d ? fmax(mass_of(pj) - mass_of(dj), 0.0) : mass_of(pj);
-        return j == only ? 0.0 : v;
+        if (d) return fmax(mass_of(pj) - mass_of(dj), 0.0);
+        return j == only ? 0.0 : mass_of(pj);
     }
 };
 
@@ -160,39 +162,53 @@ template <typename T, int G> __global__ __launch_bounds__(256) void k_verify_gro
     if (lane == 0) q.accepted[b] = n;
 }
 
-// Wide action sets: one block per sequence.  The row is cut into stretches of four wide loads of a wave; a wave sums whole
+// Wide action sets: one block per sequence.  The row is cut into stretches of two wide loads of a wave; a wave sums whole
 // stretches, the first wave finds the stretch in which the running sum passes the goal and walks that one again.
-// 256 x 100003 float32: 34 us (205 MB, 5.9 TB/s with part of the rows in cache); one sequence of 32000: 11 us, of which the
-// launch is 3 and four dependent trips to memory most of the rest.
-template <typename T> constexpr int STRETCH = 4 * 64 * (16 / (int)sizeof(T));
+// 256 x 100003 float32: 35 us (205 MB, 5.9 TB/s with part of the rows in cache); 2000 x 32000 bfloat16 97 us (256 MB, bound by
+// the float64 sums); one sequence of 32000 float32: 10 us, of which the launch is 3 and four dependent trips to memory most of
+// the rest; one of 130000: 24 us, what one compute unit can read.
+constexpr int STRETCH_LOADS = 2;
+template <typename T> constexpr int STRETCH = STRETCH_LOADS * 64 * (16 / (int)sizeof(T));
 
-template <typename T> __device__ __forceinline__ void load_stretch(const Left<T> &left, int j0, int V, double (&v)[4][16 / sizeof(T)])
-{
-    constexpr int E = 16 / sizeof(T);
-    const int lane = threadIdx.x % 64;
-    Loose<T, E> p[4], d[4];
-    if (j0 + STRETCH<T> <= V) {
+template <typename T> struct StretchOf {
+    static constexpr int E = 16 / sizeof(T), N = STRETCH_LOADS;
+    Loose<T, E> p[N], d[N];
+
+    __device__ __forceinline__ void load(const Left<T> &left, int j0, int V)
+    {
+        const int lane = threadIdx.x % 64;
+        if (j0 + STRETCH<T> <= V) {
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const int j = j0 + (i * 64 + lane) * E;
-            p[i] = *(const Loose<T, E> *)(left.p + j);
-            if (left.d) d[i] = *(const Loose<T, E> *)(left.d + j);
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < 4; i++)
-#pragma unroll
-            for (int e = 0; e < E; e++) {
-                const int j = j0 + (i * 64 + lane) * E + e;
-                p[i].v[e] = j < V ? left.p[j] : T(0.0f);
-                d[i].v[e] = left.d && j < V ? left.d[j] : T(0.0f);
+            for (int i = 0; i < N; i++) {
+                const int j = j0 + (i * 64 + lane) * E;
+                p[i] = *(const Loose<T, E> *)(left.p + j);
+                if (left.d) d[i] = *(const Loose<T, E> *)(left.d + j);
             }
+        } else {
+#pragma unroll
+            for (int i = 0; i < N; i++)
+#pragma unroll
+                for (int e = 0; e < E; e++) {
+                    const int j = j0 + (i * 64 + lane) * E + e;
+                    p[i].v[e] = j < V ? left.p[j] : T(0.0f);
+                    d[i].v[e] = left.d && j < V ? left.d[j] : T(0.0f);
+                }
+        }
     }
+    __device__ __forceinline__ double at(const Left<T> &left, int j0, int i, int e) const
+    {
+        return left.of(p[i].v[e], left.d ? d[i].v[e] : T(0.0f), j0 + (i * 64 + (int)(threadIdx.x % 64)) * E + e);
+    }
+    __device__ __forceinline__ double sum(const Left<T> &left, int j0) const
+    {
+        double s = 0;
 #pragma unroll
-    for (int i = 0; i < 4; i++)
+        for (int i = 0; i < N; i++)
 #pragma unroll
-        for (int e = 0; e < E; e++) v[i][e] = left.of(p[i].v[e], left.d ? d[i].v[e] : T(0.0f), j0 + (i * 64 + lane) * E + e);
-}
+            for (int e = 0; e < E; e++) s += at(left, j0, i, e);
+        return group_sum<64>(s);
+    }
+};
 
 template <typename T> __global__ __launch_bounds__(1024) void k_verify(VerifyArgs q)
 {
@@ -210,15 +226,16 @@ template <typename T> __global__ __launch_bounds__(1024) void k_verify(VerifyArg
     Left<T> left(q, b, n, length);
     int token = -1;
     while (true) {
-        for (int i = w; i < stretches; i += nw) {
-            double v[4][E], s = 0;
-            load_stretch(left, i * STRETCH<T>, q.V, v);
+        constexpr int AHEAD = 2;   // stretches of a wave on their way at a time (four: 1 x 130000 float32 26 instead of 24 us)
+        for (int i = w; i < stretches; i += AHEAD * nw) {
+            StretchOf<T> some[AHEAD];
 #pragma unroll
-            for (int a = 0; a < 4; a++)
+            for (int u = 0; u < AHEAD; u++) some[u].load(left, min(i + u * nw, stretches - 1) * STRETCH<T>, q.V);
 #pragma unroll
-                for (int e = 0; e < E; e++) s += v[a][e];
-            s = group_sum<64>(s);
-            if (lane == 0) part[i] = s;
+            for (int u = 0; u < AHEAD; u++) {
+                const double s = some[u].sum(left, min(i + u * nw, stretches - 1) * STRETCH<T>);
+                if (lane == 0 && i + u * nw < stretches) part[i + u * nw] = s;
+            }
         }
         __syncthreads();
         if (w == 0) {
@@ -241,22 +258,22 @@ template <typename T> __global__ __launch_bounds__(1024) void k_verify(VerifyArg
             if (hi >= 0) {   // the row has mass
                 const int s = lo < 64 ? __shfl(pick, lo) : __shfl(last, hi);
                 double below = lo < 64 ? __shfl(pick_at, lo) : __shfl(last_at, hi);
-                double v[4][E];
-                load_stretch(left, s * STRETCH<T>, q.V, v);
+                StretchOf<T> walk;
+                walk.load(left, s * STRETCH<T>, q.V);
                 int end = -1;
 #pragma unroll
-                for (int a = 0; a < 4; a++) {
-                    double mine = 0, c[E];
+                for (int a = 0; a < STRETCH_LOADS; a++) {
+                    double mine = 0, c[E], v[E];
 #pragma unroll
-                    for (int e = 0; e < E; e++) mine += v[a][e], c[e] = mine;
+                    for (int e = 0; e < E; e++) v[e] = walk.at(left, s * STRETCH<T>, a, e), mine += v[e], c[e] = mine;
                     const double incl = running_sum<64>(mine, lane);
                     double before = __shfl_up(incl, 1);
                     if (lane == 0) before = 0;
                     int hit = -1, some = -1;
 #pragma unroll
                     for (int e = E - 1; e >= 0; e--) {
-                        if (v[a][e] > 0 && below + (before + c[e]) > goal) hit = e;
-                        if (v[a][e] > 0 && some < 0) some = e;
+                        if (v[e] > 0 && below + (before + c[e]) > goal) hit = e;
+                        if (v[e] > 0 && some < 0) some = e;
                     }
                     const int l = lowest_lane<64>(hit >= 0), h = highest_lane<64>(some >= 0);
                     const int base = s * STRETCH<T> + a * 64 * E;
