@@ -431,7 +431,11 @@ typedef struct mz_strided {
  * last position (may be NULL).
  * mz_linear_recurrence_backward: gate as before, x = gradient of out -> out = gradient of x; with y = the outputs,
  * out_gate = gradient of gate (both or neither; state as before); grad_last = gradient of last (NULL: 0), out_state =
- * gradient of state (may be NULL).  Inputs and outputs must not overlap. */
+ * gradient of state (may be NULL).  Inputs and outputs must not overlap.
+ * fine, for 16-bit tensors whose gate wants a gradient: device bytes in which the forward call keeps what the rounding of out
+ * lost and which the backward call reads with y, so that the gate's gradient is rounded once (p = NULL: y as stored, about 1.4
+ * roundings).  The byte of the s-th position in the order of the FORWARD pass lies at p + b * stride_b + s / 4 * stride_t +
+ * d * stride_d + s % 4; p and the strides (in bytes) are multiples of 4, and whole words of four positions are written. */
 typedef struct mz_recurrence {
     int32_t type, B, D, reverse;   /* B * D at most 2^30 */
     int64_t T;
@@ -442,6 +446,7 @@ typedef struct mz_recurrence {
     void *out_state;
     void *workspace;           /* device memory of this call alone, 64-byte aligned, or NULL where none is needed */
     int64_t workspace_bytes;
+    mz_strided fine;           /* not looked at for MZ_F32 and MZ_F64 */
 } mz_recurrence;
 /* Device bytes a call with these arguments needs as workspace (0 up to T = 256; backward != 0: of the backward call). */
 int mz_linear_recurrence_workspace(const mz_recurrence *args_h, int32_t backward, int64_t *out_bytes);

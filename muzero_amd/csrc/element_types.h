@@ -14,6 +14,30 @@ template <typename T> __device__ __forceinline__ acc_t<T> widen(T v) { return (a
 // One rounding to nearest even, at the store (v_cvt_pk_bf16_f32 / v_cvt_f16_f32 on gfx950).
 template <typename T> __device__ __forceinline__ T narrow(acc_t<T> v) { return (T)v; }
 
+// What a rounding to 16 bits lost, in 8 more bits: the distance of the float32 pattern from that of the rounded value (patterns
+// of one sign are ordered like their values, across exponents too) in steps of 2^FINE_SHIFT, held in byte FINE_BYTE of what
+// fine_of() returns.  refined() is then within one such step of the float32 value, 2^-15 of it (bfloat16) or 2^-18 (float16).
+// A bfloat16 has float32's exponents: half a step of its own is 2^15 everywhere, what rounds to infinity comes back finite, and
+// adding up to 2^15 to a quiet NaN leaves one.  A float16 among its subnormal numbers is off by more than fits and is never
+// further off than the rounded value; its infinities and NaN are left as they are.
+template <typename T> constexpr int FINE_SHIFT = 8;
+template <> constexpr int FINE_SHIFT<_Float16> = 5;
+__device__ __forceinline__ int pattern(float v) { return __builtin_bit_cast(int, v); }
+__device__ __forceinline__ unsigned fine_of(float v, __bf16 rounded)   // in byte 1
+{
+    return (unsigned)(min(pattern(v) - pattern((float)rounded), 0x7f7f) + 0x80);
+}
+__device__ __forceinline__ unsigned fine_of(float v, _Float16 rounded)
+{
+    const int w = pattern((float)rounded), d = min(max(pattern(v) - w, -0x1000), 0xfef) + 0x10;
+    return (w & 0x7f800000) == 0x7f800000 ? 0u : (unsigned)d << 3;
+}
+template <typename A, typename T> __device__ __forceinline__ unsigned fine_of(A, T) { return 0; }
+template <typename T> __device__ __forceinline__ float refined(T rounded, signed char fine)
+{
+    return __builtin_bit_cast(float, pattern((float)rounded) + (int)fine * (1 << FINE_SHIFT<T>));
+}
+
 __device__ __forceinline__ float fma_acc(float a, float b, float c) { return __builtin_fmaf(a, b, c); }
 __device__ __forceinline__ double fma_acc(double a, double b, double c) { return __builtin_fma(a, b, c); }
 

@@ -50,6 +50,8 @@ static RecurrencePlan plan_recurrence(const mz_recurrence *a, bool backward)
         if (t->stride_d != 1) p.channels = false;
         low |= (uint64_t)(uintptr_t)t->p | (uint64_t)t->stride_b * size | (uint64_t)t->stride_t * size;
     }
+    if (size == 2 && a->fine.p)   // four bytes a channel where the others have two; only neighbouring ones travel together
+        low |= (((uint64_t)(uintptr_t)a->fine.p | (uint64_t)a->fine.stride_b | (uint64_t)a->fine.stride_t) >> 1) | (a->fine.stride_d != 4 ? 2 : 0);
     if (a->D == 1) p.channels = false;
     if (!p.channels) {
         const long long links = (a->T + ROW_LINK - 1) / ROW_LINK;
@@ -146,6 +148,8 @@ static int check_recurrence(const mz_recurrence *a, bool backward, const char *f
     if (!a->gate.p || !a->x.p || !a->out.p) return api_fail(MZ_ERR_ARG, std::string(fn) + ": null tensor");
     if (backward && (a->out_gate.p != nullptr) != (a->y.p != nullptr))
         return api_fail(MZ_ERR_ARG, std::string(fn) + ": the gates' gradient needs the outputs, and nothing else does");
+    if (size_of(a->type) == 2 && a->fine.p && ((uintptr_t)a->fine.p | (uint64_t)a->fine.stride_b | (uint64_t)a->fine.stride_t | (uint64_t)a->fine.stride_d) % 4 != 0)
+        return api_fail(MZ_ERR_ARG, std::string(fn) + ": fine and its strides must be multiples of 4 bytes");
     return MZ_OK;
 }
 
@@ -167,6 +171,7 @@ template <bool BWD> static int run_recurrence(const mz_recurrence *a, void *stre
     };
     q.a = view(a->gate), q.x = view(a->x), q.out = view(a->out);
     if (BWD) q.y = view(a->y), q.da = view(a->out_gate), q.state0 = a->y.p ? a->state : nullptr;
+    if (size_of(a->type) == 2 && (!BWD || a->y.p)) q.fine = {a->fine.p, a->fine.stride_b, a->fine.stride_t, a->fine.stride_d};
     q.first = BWD ? a->grad_last : a->state, q.last = BWD ? a->out_state : a->last;
     hipStream_t st = (hipStream_t)stream;
     switch (a->type) {

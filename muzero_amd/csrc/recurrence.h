@@ -22,6 +22,9 @@ struct RecurrenceArgs {
     View a, x;           // gates and inputs (backward: dy)
     View y;              // backward: the forward pass's outputs, or p = NULL where no gate gradient is wanted
     View out, da;        // y (backward: dx), gate gradients
+    // What y's rounding to 16 bits lost (fine_of), a byte a position of the FORWARD pass's scan order: position s lies at
+    // p + b * sb + s / 4 * st + d * sd + s % 4.  p = NULL: not kept.
+    View fine;
     const void *first;   // acc[B][D] what goes into position 0 (backward: gradient of the last state), NULL = 0
     const void *state0;  // backward: acc[B][D] the forward pass's first state, NULL = 0
     void *last;          // acc[B][D] the state behind the last position (backward: gradient of the first state), may be NULL
@@ -36,10 +39,99 @@ template <typename T> __device__ __forceinline__ const T *at(const RecurrenceArg
 
 template <typename A> __device__ __forceinline__ A state_at(const void *p, long long i) { return p ? ((const A *)p)[i] : A(0); }
 
+// The bytes of `fine` that L positions need, in words of four positions each: 4 x 8192 x 4096 bfloat16 in 243 us forward and 315
+// backward (199 and 294 without them); a load or store of two bytes a lane for every position took 248 and 398.
+template <int VEC, int L> struct Fine {
+    using W = Pack<unsigned, VEC>;
+    W w[L / 4 + 1];
+    static __device__ __forceinline__ W *word(const RecurrenceArgs &q, int b, long long k, int d)
+    {
+        return (W *)((char *)q.fine.p + (long long)b * q.fine.sb + k * q.fine.st + (long long)d * q.fine.sd);
+    }
+    // Backward: those of what precedes the L positions from s0 on, the forward pass's T - 2 - s0 and the ones in front of it.
+    __device__ __forceinline__ void load(const RecurrenceArgs &q, int b, long long s0, int d)
+    {
+        const long long k = (q.T - 1 - s0 - L) >> 2, last = (q.T - 1) >> 2;   // a word outside 0 .. last holds no position that is used
+        if (!q.fine.p) {
+#pragma unroll
+            for (int j = 0; j <= L / 4; j++) w[j] = W{};
+            return;
+        }
+        const char *at = (const char *)word(q, b, min(max(k, 0ll), last), d);
+#pragma unroll
+        for (int j = 0; j <= L / 4; j++) {
+            w[j] = *(const W *)at;
+            if (k + j >= 0 && k + j < last) at += q.fine.st;
+        }
+    }
+    __device__ __forceinline__ void line_up(const RecurrenceArgs &q)   // lets the last of the L positions begin a word
+    {
+        const unsigned shift = (unsigned)(q.T - 1 - L) & 3;   // s0 is a multiple of 4
+#pragma unroll
+        for (int j = 0; j < L / 4; j++)
+#pragma unroll
+            for (int v = 0; v < VEC; v++) w[j].v[v] = __builtin_amdgcn_alignbyte(w[j + 1].v[v], w[j].v[v], shift);
+    }
+    __device__ __forceinline__ signed char at(int i, int v) const { return (signed char)(w[(L - 1 - i) / 4].v[v] >> (L - 1 - i) % 4 * 8); }
+    // Forward: byte 1 of `fine` for position s0 + i, in order, and all of them together.
+    __device__ __forceinline__ void put(int i, int v, unsigned fine)
+    {
+        // v_perm: bytes 0 .. 3 are those of the second operand, 4 .. 7 those of the first, 12 is zero
+        constexpr unsigned at[4] = {0x0c0c0c05u, 0x0c0c0500u, 0x0c050100u, 0x05020100u};
+        w[i / 4].v[v] = __builtin_amdgcn_perm(fine, i % 4 ? w[i / 4].v[v] : 0u, at[i % 4]);
+    }
+    __device__ __forceinline__ void store(const RecurrenceArgs &q, int b, long long s0, int d, int left) const
+    {
+#pragma unroll
+        for (int j = 0; j < L / 4; j++) if (4 * j < left) *word(q, b, (s0 >> 2) + j, d) = w[j];
+    }
+};
+// ... of fewer than four positions: byte by byte.
+template <int VEC> struct Fine<VEC, 2> {
+    signed char f[2];
+    static __device__ __forceinline__ signed char *byte(const RecurrenceArgs &q, int b, long long s, int d)
+    {
+        return (signed char *)q.fine.p + (long long)b * q.fine.sb + (s >> 2) * q.fine.st + (long long)d * q.fine.sd + (s & 3);
+    }
+    __device__ __forceinline__ void load(const RecurrenceArgs &q, int b, long long s0, int d)
+    {
+#pragma unroll
+        for (int i = 0; i < 2; i++) f[i] = q.fine.p ? *byte(q, b, max(q.T - 2 - s0 - i, 0ll), d) : 0;
+    }
+    __device__ __forceinline__ void line_up(const RecurrenceArgs &) {}
+    __device__ __forceinline__ signed char at(int i, int) const { return f[i]; }
+    __device__ __forceinline__ void put(int i, int, unsigned fine) { f[i] = (signed char)(fine >> 8); }
+    __device__ __forceinline__ void store(const RecurrenceArgs &q, int b, long long s0, int d, int left) const
+    {
+#pragma unroll
+        for (int i = 0; i < 2; i++) if (i < left) *byte(q, b, s0 + i, d) = f[i];
+    }
+};
+// 32- and 64-bit tensors keep nothing of the kind.
+struct NoFine {
+    __device__ __forceinline__ void load(const RecurrenceArgs &, int, long long, int) {}
+    __device__ __forceinline__ void line_up(const RecurrenceArgs &) {}
+    __device__ __forceinline__ signed char at(int, int) const { return 0; }
+    __device__ __forceinline__ void put(int, int, unsigned) {}
+    __device__ __forceinline__ void store(const RecurrenceArgs &, int, long long, int, int) const {}
+};
+template <typename T, int VEC, int L> struct FineOf { using type = Fine<VEC, L>; };
+template <int VEC, int L> struct FineOf<float, VEC, L> { using type = NoFine; };
+template <int VEC, int L> struct FineOf<double, VEC, L> { using type = NoFine; };
+
+// What precedes a position, for its gate's gradient: the forward pass's state there as y and fine hold it.
+template <typename T> __device__ __forceinline__ acc_t<T> before_of(T y, signed char fine)
+{
+    if constexpr (sizeof(T) == 2) return refined(y, fine);
+    else return widen(y);
+}
+
 // L positions of one strand in registers, all loads asked for at once.
 template <typename T, int VEC, int L, bool BWD> struct Strand {
     using P = Pack<T, VEC>;
+    using F = typename FineOf<T, VEC, L>::type;
     P a[L], x[L], y[BWD ? L : 1];
+    F f;   // forward: empty until the walk
 
     // FULL: every position is below the end (and, backward, so is the one behind it); otherwise addresses are clamped and
     // positions from `end` on become the identity map.
@@ -67,12 +159,17 @@ template <typename T, int VEC, int L, bool BWD> struct Strand {
 #pragma unroll
                     for (int j = 0; j < VEC; j++) a[i].v[j] = T(1.0f), x[i].v[j] = T(0.0f);
     }
-    // The strand's outputs from the state h in front of it: each y (dx) rounded once from the 32- or 64-bit state, a gate's
-    // gradient from that state and the stored, once rounded y - keeping y in 32 bits as well would cost a training step of
-    // 16-bit tensors two more bytes an element each way for half a bit of one gradient.
-    __device__ __forceinline__ void walk(const RecurrenceArgs &q, int b, long long s0, long long end, int d, bool want_da, acc_t<T> (&h)[VEC]) const
+    __device__ __forceinline__ void load_fine(const RecurrenceArgs &q, int b, long long s0, int d, bool want_da)
+    {
+        if (BWD && want_da) f.load(q, b, s0, d);
+    }
+    // The strand's outputs from the state h in front of it, each rounded once from the 32- or 64-bit state.  A gate's gradient
+    // multiplies two states: of 16-bit tensors the forward pass keeps 8 bits of what y's rounding lost beside it (one more byte
+    // an element each way), since the stored y alone made that gradient's error 1.4 times a rounding.
+    __device__ __forceinline__ void walk(const RecurrenceArgs &q, int b, long long s0, long long end, int d, bool want_da, acc_t<T> (&h)[VEC])
     {
         using A = acc_t<T>;
+        if (BWD && want_da) f.line_up(q);
         const int left = (int)min((long long)L, max(end - s0, 0ll));
 #pragma unroll
         for (int i = 0; i < L; i++) {
@@ -84,17 +181,25 @@ template <typename T, int VEC, int L, bool BWD> struct Strand {
                 o.v[j] = narrow<T>(h[j]);
             }
             *(P *)at<T>(q.out, b, s0 + i, d) = o;
+            if constexpr (!BWD && sizeof(T) == 2) {
+                if (q.fine.p)
+#pragma unroll
+                    for (int j = 0; j < VEC; j++) f.put(i, j, fine_of(h[j], o.v[j]));
+            }
             if constexpr (BWD) {
                 if (want_da) {
                     const bool first = s0 + i + 1 == q.T;   // of the forward pass: what precedes it is the first state
 #pragma unroll
                     for (int j = 0; j < VEC; j++) {
-                        const A before = first ? state_at<A>(q.state0, (long long)b * q.D + d + j) : widen(y[i].v[j]);
+                        const A before = first ? state_at<A>(q.state0, (long long)b * q.D + d + j) : before_of<T>(y[i].v[j], f.at(i, j));
                         da.v[j] = narrow<T>(h[j] * before);
                     }
                     *(P *)at<T>(q.da, b, s0 + i, d) = da;
                 }
             }
+        }
+        if constexpr (!BWD) {
+            if (q.fine.p) f.store(q, b, s0, d, left);
         }
     }
     // The strand's map behind the map (ra, rx).
@@ -153,6 +258,7 @@ __global__ __launch_bounds__(REC_THREADS) void k_recurrence_channels(RecurrenceA
     auto load = [&](Strand<T, VEC, L, BWD> &w, long long base) {
         if (base + round <= inside) w.template load<true>(q, b, base + v * L, end, d, want_da);
         else w.template load<false>(q, b, base + v * L, end, d, want_da);
+        w.load_fine(q, b, base + v * L, d, want_da);
     };
     load(now, 0);
     for (long long base = 0; base < end; base += round, buf ^= 1) {
@@ -198,7 +304,7 @@ __global__ __launch_bounds__(REC_THREADS) void k_recurrence_channels(RecurrenceA
 // and that wait for earlier ones in turn: every wait ends.
 // 50000 x 1000 float32 in 140 us (600 MB, 4.3 TB/s) and 5 us for the granules; reading the inputs once for the maps and once for
 // the outputs instead took 211 us, links of half the positions 150, asking four predecessors at once 142 (registers spill).
-// The gradients of 4 x 8192 x 4096 bfloat16 in 294 us (five tensors, 4.6 TB/s) and 7 for the granules.
+// The gradients of 4 x 8192 x 4096 bfloat16 in 315 us (five tensors and a byte an element, 4.7 TB/s) and 7 for the granules.
 constexpr int CHAIN_BACK = 16;
 constexpr int CHAIN_LENGTH(int size) { return size == 8 ? 8 : 16; }   // positions of a wave; float64 takes twice the registers
 constexpr int CHAIN_WAVES(int size, bool backward) { return backward && size != 8 ? 8 : 16; }   // backward: a third tensor in registers
@@ -315,6 +421,8 @@ __global__ __launch_bounds__(64 * CHAIN_WAVES(sizeof(T), BWD)) void k_recurrence
             }
         }
     }
+    // Not before the look back: held across it, they take the registers past 128 and with that half of the waves of a unit.
+    w.load_fine(q, b, s0, d, want_da);
     lds_fence_barrier();
     const State before = front[c];
     A h[VEC];
@@ -348,6 +456,7 @@ __global__ __launch_bounds__(256) void k_recurrence_short(RecurrenceArgs q)
     for (long long s0 = 0; s0 < q.T; s0 += L) {
         Strand<T, VEC, L, BWD> w;
         w.template load<false>(q, b, s0, q.T, d, want_da);
+        w.load_fine(q, b, s0, d, want_da);
         w.walk(q, b, s0, q.T, d, want_da, h);
     }
     if (q.last)
@@ -397,12 +506,13 @@ __global__ __launch_bounds__(1024) void k_recurrence_rows(RecurrenceArgs q)
     for (long long base = 0; base < q.T; base += (long long)blockDim.x * E, buf ^= 1) {
         const long long s0 = base + (long long)threadIdx.x * E;
         Stretch<T, E> a, x, y;
+        typename FineOf<T, 1, E>::type f;
         x.load(q.x, at<T>(q.x, b, 0, d), s0, q.T, T(0.0f));
         // a position behind the end is the identity map; backward, the one in front of the first as well
         if (!BWD) a.load(q.a, at<T>(q.a, b, 0, d), s0, q.T, T(1.0f));
         else {
             a.load(q.a, at<T>(q.a, b, 0, d), s0 - 1, q.T, T(1.0f));
-            if (want_da) y.load(q.y, at<T>(q.y, b, 0, d), s0 + 1, q.T, T(0.0f));
+            if (want_da) y.load(q.y, at<T>(q.y, b, 0, d), s0 + 1, q.T, T(0.0f)), f.load(q, b, s0, d), f.line_up(q);
             if (s0 + E > q.T)
 #pragma unroll
                 for (int i = 0; i < E; i++) if (s0 + i >= q.T) a.v[i] = T(1.0f);
@@ -432,10 +542,11 @@ __global__ __launch_bounds__(1024) void k_recurrence_rows(RecurrenceArgs q)
             h = fma_acc(widen(a.v[i]), h, widen(x.v[i]));
             o.v[i] = narrow<T>(h);
             if constexpr (BWD) {
-                if (want_da) da.v[i] = narrow<T>(h * (s0 + i + 1 == q.T ? state_at<A>(q.state0, blockIdx.x) : widen(y.v[i])));
-            }
+                if (want_da) da.v[i] = narrow<T>(h * (s0 + i + 1 == q.T ? state_at<A>(q.state0, blockIdx.x) : before_of<T>(y.v[i], f.at(i, 0))));
+            } else if (sizeof(T) == 2) f.put(i, 0, fine_of(h, o.v[i]));
         }
         o.store(q.out, (T *)at<T>(q.out, b, 0, d), s0, q.T);
+        if (!BWD && q.fine.p) f.store(q, b, s0, d, (int)min((long long)E, q.T - s0));
         if constexpr (BWD) {
             if (want_da) da.store(q.da, (T *)at<T>(q.da, b, 0, d), s0, q.T);
         }
@@ -464,11 +575,12 @@ __global__ __launch_bounds__(1024) void k_recurrence_row_chain(RecurrenceArgs q)
     const bool want_da = BWD && q.da.p;
     const long long s0 = (long long)link * ROW_LINK + threadIdx.x * E;
     Stretch<T, E> a, x, y;
+    typename FineOf<T, 1, E>::type f;
     x.load(q.x, at<T>(q.x, b, 0, d), s0, q.T, T(0.0f));
     if (!BWD) a.load(q.a, at<T>(q.a, b, 0, d), s0, q.T, T(1.0f));
     else {
         a.load(q.a, at<T>(q.a, b, 0, d), s0 - 1, q.T, T(1.0f));
-        if (want_da) y.load(q.y, at<T>(q.y, b, 0, d), s0 + 1, q.T, T(0.0f));
+        if (want_da) y.load(q.y, at<T>(q.y, b, 0, d), s0 + 1, q.T, T(0.0f)), f.load(q, b, s0, d), f.line_up(q);
         if (s0 + E > q.T)
 #pragma unroll
             for (int i = 0; i < E; i++) if (s0 + i >= q.T) a.v[i] = T(1.0f);
@@ -529,10 +641,11 @@ __global__ __launch_bounds__(1024) void k_recurrence_row_chain(RecurrenceArgs q)
         h = fma_acc(widen(a.v[i]), h, widen(x.v[i]));
         o.v[i] = narrow<T>(h);
         if constexpr (BWD) {
-            if (want_da) da.v[i] = narrow<T>(h * (s0 + i + 1 == q.T ? state_at<A>(q.state0, row) : widen(y.v[i])));
-        }
+            if (want_da) da.v[i] = narrow<T>(h * (s0 + i + 1 == q.T ? state_at<A>(q.state0, row) : before_of<T>(y.v[i], f.at(i, 0))));
+        } else if (sizeof(T) == 2) f.put(i, 0, fine_of(h, o.v[i]));
     }
     o.store(q.out, (T *)at<T>(q.out, b, 0, d), s0, q.T);
+    if (!BWD && q.fine.p) f.store(q, b, s0, d, (int)min((long long)E, q.T - s0));
     if constexpr (BWD) {
         if (want_da) da.store(q.da, (T *)at<T>(q.da, b, 0, d), s0, q.T);
     }

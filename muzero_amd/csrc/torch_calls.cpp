@@ -70,8 +70,9 @@ static bool by_channels(const Tensor &x) { return x.size(2) > 1 && (x.stride(2) 
 
 static at::TensorOptions wide(const Tensor &x) { return x.options().dtype(x.scalar_type() == at::kDouble ? at::kDouble : at::kFloat); }
 
+// fine: [B, positions / 4, D, 4] bytes, undefined where nothing is kept
 static void run_recurrence(bool backward, Tensor gate, Tensor x, const Tensor &state, bool reverse, Tensor out, Tensor y, Tensor out_gate,
-                           const Tensor &last, const Tensor &grad_last, const Tensor &out_state, int64_t stream)
+                           const Tensor &last, const Tensor &grad_last, const Tensor &out_state, Tensor fine, int64_t stream)
 {
     mz_recurrence a{};
     int64_t B = x.size(0), T = x.size(1), D = x.size(2);
@@ -82,6 +83,7 @@ static void run_recurrence(bool backward, Tensor gate, Tensor x, const Tensor &s
         for (Tensor *v : views) all &= !v->defined() || v->stride(0) == 1;
         if (all) {
             for (Tensor *v : views) if (v->defined()) *v = v->transpose(0, 2);
+            if (fine.defined()) fine = fine.transpose(0, 2);
             D = B, B = 1;
         }
     }
@@ -91,6 +93,7 @@ static void run_recurrence(bool backward, Tensor gate, Tensor x, const Tensor &s
     TORCH_CHECK_VALUE(B <= INT32_MAX && D <= INT32_MAX, "linear_recurrence: sizes must be positive, and B * D at most 2^30");
     a.type = type_of(x), a.B = (int32_t)B, a.D = (int32_t)D, a.T = T, a.reverse = reverse;
     a.state = ptr(state), a.last = ptr(last), a.grad_last = ptr(grad_last), a.out_state = ptr(out_state);
+    if (fine.defined()) a.fine = {fine.data_ptr(), fine.stride(0), fine.stride(1), fine.stride(2)};
     Tensor space;
     if (T > 256) {   // shorter records need none
         check(entry.recurrence_workspace(&a, backward, &a.workspace_bytes));
@@ -103,14 +106,22 @@ static void run_recurrence(bool backward, Tensor gate, Tensor x, const Tensor &s
     check((backward ? entry.recurrence_backward : entry.recurrence)(&a, reinterpret_cast<void *>(stream)));
 }
 
-static std::tuple<Tensor, Tensor> recurrence_forward(const Tensor &gate, const Tensor &x, const Tensor &state, bool reverse, int64_t stream)
+// y, the last state, and with keep what the rounding of a 16-bit y lost
+static std::tuple<Tensor, Tensor, Tensor> recurrence_forward(const Tensor &gate, const Tensor &x, const Tensor &state, bool reverse, bool keep, int64_t stream)
 {
-    if (x.numel() == 0) return {at::empty_like(x), state.defined() ? state.clone() : at::zeros({x.size(0), x.size(2)}, wide(x))};
+    if (x.numel() == 0) return {at::empty_like(x), state.defined() ? state.clone() : at::zeros({x.size(0), x.size(2)}, wide(x)), {}};
     const bool channels = by_channels(x);
     const Tensor xl = lined_up(x, channels);
     Tensor y = like(xl, channels), last = at::empty({x.size(0), x.size(2)}, wide(x));
-    run_recurrence(false, lined_up(gate, channels), xl, state, reverse, y, {}, {}, last, {}, {}, stream);
-    return {y, last};
+    Tensor fine;
+    if (keep && x.element_size() == 2) {   // as close together as y's elements
+        const int64_t B = x.size(0), words = (x.size(1) + 3) / 4, D = x.size(2);
+        const auto bytes = x.options().dtype(at::kChar);
+        fine = channels ? at::empty({B, words, D, 4}, bytes)
+             : D == 1 && y.stride(0) == 1 ? at::empty({words, B, D, 4}, bytes).transpose(0, 1) : at::empty({B, D, words, 4}, bytes).transpose(1, 2);
+    }
+    run_recurrence(false, lined_up(gate, channels), xl, state, reverse, y, {}, {}, last, {}, {}, fine, stream);
+    return {y, last, fine};
 }
 
 struct Recurrence : torch::autograd::Function<Recurrence> {
@@ -118,11 +129,11 @@ struct Recurrence : torch::autograd::Function<Recurrence> {
                                  int64_t stream)
     {
         const Tensor state = first.value_or(Tensor());
-        auto [y, last] = recurrence_forward(gate, x, state, reverse, stream);
+        auto [y, last, fine] = recurrence_forward(gate, x, state, reverse, gate.requires_grad(), stream);
         ctx->set_materialize_grads(false);
         ctx->saved_data["reverse"] = reverse;
         ctx->saved_data["stream"] = stream;
-        ctx->save_for_backward({gate, gate.requires_grad() ? y : Tensor(), state});
+        ctx->save_for_backward({gate, gate.requires_grad() ? y : Tensor(), state, fine});
         return {y, last};
     }
     static variable_list backward(AutogradContext *ctx, variable_list grads)
@@ -130,7 +141,7 @@ struct Recurrence : torch::autograd::Function<Recurrence> {
         Tensor dy = grads[0], dlast = grads[1];
         if (!dy.defined() && !dlast.defined()) return {{}, {}, {}, {}, {}};
         const auto saved = ctx->get_saved_variables();
-        Tensor gate = saved[0].detach(), y = saved[1], state = saved[2];
+        Tensor gate = saved[0].detach(), y = saved[1], state = saved[2], fine = saved[3];
         const bool want_gate = ctx->needs_input_grad(0), want_x = ctx->needs_input_grad(1), want_state = state.defined() && ctx->needs_input_grad(2);
         variable_list out(5);
         {
@@ -147,7 +158,7 @@ struct Recurrence : torch::autograd::Function<Recurrence> {
                 dy = lined_up(dy, channels);
                 Tensor dx = like(dy, channels), dgate = want_gate ? like(dy, channels) : Tensor();
                 run_recurrence(true, lined_up(gate, channels), dy, state, ctx->saved_data["reverse"].toBool(), dx,
-                               want_gate ? lined_up(y, channels) : Tensor(), dgate, {}, dlast, dstate, ctx->saved_data["stream"].toInt());
+                               want_gate ? lined_up(y, channels) : Tensor(), dgate, {}, dlast, dstate, fine, ctx->saved_data["stream"].toInt());
                 out[0] = dgate, out[1] = want_x ? dx : Tensor(), out[2] = dstate;
             }
         }
@@ -162,7 +173,8 @@ static std::tuple<Tensor, Tensor> linear_recurrence(const Tensor &gate, const Te
         auto out = Recurrence::apply(gate, x, s.defined() ? std::optional<Tensor>(s) : std::nullopt, reverse, stream);
         return {out[0], out[1]};
     }
-    return recurrence_forward(gate, x, s, reverse, stream);
+    auto [y, last, fine] = recurrence_forward(gate, x, s, reverse, false, stream);
+    return {y, last};
 }
 
 // ------------------------------------------------------------------------------------------------ distillation

@@ -62,7 +62,7 @@ class MzRecurrence(C.Structure):
     _fields_ = [('type', C.c_int32), ('B', C.c_int32), ('D', C.c_int32), ('reverse', C.c_int32), ('T', C.c_int64),
                 ('gate', MzStrided), ('x', MzStrided), ('out', MzStrided), ('y', MzStrided), ('out_gate', MzStrided),
                 ('state', C.c_void_p), ('last', C.c_void_p), ('grad_last', C.c_void_p), ('out_state', C.c_void_p),
-                ('workspace', C.c_void_p), ('workspace_bytes', C.c_int64)]
+                ('workspace', C.c_void_p), ('workspace_bytes', C.c_int64), ('fine', MzStrided)]
 
 
 class MzDistill(C.Structure):
