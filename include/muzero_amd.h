@@ -456,8 +456,9 @@ int mz_linear_recurrence_backward(const mz_recurrence *args_h, void *stream);
 /* Distillation of a policy from a teacher's top logits: loss[r] = weight[r] * temperature^2 * KL(p || q), q =
  * softmax(logits / temperature) over the V actions; p = softmax(teacher / temperature) over the K entries, or, with lse
  * (log-sum-exp of the teacher's logits / temperature over all actions), p = exp(teacher / temperature - lse) and one more
- * class of all actions outside the entries (left out where the student gives those nothing).  The soft cross-entropy the
- * trainer takes over whole rows (trainer.py:119-122), for targets that name few actions.
+ * class of all actions outside the entries (left out where all of those are masked: logits of -inf, or of the type's lowest
+ * value and next to nothing).  The soft cross-entropy the trainer takes over whole rows (trainer.py:119-122), for targets that
+ * name few actions.
  * Entries whose index lies outside 0..V-1 are absent; an action named twice gets the sum.  Rows without entries and
  * rows of weight 0 have loss and gradient 0 whatever their logits hold.
  * mz_distill_loss: loss and stats.  mz_distill_grad: grad = grad_loss[r] * d loss[r] / d logits from those stats.

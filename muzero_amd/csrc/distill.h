@@ -24,7 +24,9 @@ struct DistillArgs {
     const float *up;         // [R] gradient of the loss, or NULL: 1
     float *loss;             // [R] or NULL
     void *grad;              // [R][V] contiguous, or NULL
-    float *stats;            // [R][4] maximum, sum, tail sum: written by the loss pass, read by a later gradient pass
+    // [R][4] maximum, sum (0: nothing of the row counts), sum outside the entries and what that one is relative to: written by
+    // the loss pass, read by a later gradient pass
+    float *stats;
     int R, V, K;
     int index64, teacher_type;
     float tau;
@@ -98,14 +100,31 @@ __device__ __forceinline__ Mass weigh(const DistillArgs &q, long long row, const
 // temperature by 2^-25 of itself, and a -inf logit stays at 0.
 __device__ __forceinline__ float expo(float d, float c) { return __builtin_amdgcn_exp2f(d * c); }
 
-// The divergence, in lane 0 of G: cross = sum p (z - m) / tau; dsum, dtail: sums of the student's exponentials over all
-// actions and over those outside the entries.  Three logarithms, taken by three lanes at once.
-template <int G>
-__device__ __forceinline__ double divergence(const Mass &e, double cross, double dsum, double ratio, int lane)
+// Exponentials of the actions outside the entries are summed relative to the row's maximum m, as all others, where that leaves
+// TAIL_LEAST or more.  Below, float32 runs out of exponents (nothing is left of an action 87 tau under the maximum) and the
+// gradient's factor rest / sum grows towards overflow: the sum is then taken again relative to the largest logit outside, mt.
+// Logits of -inf and of the type's lowest value are masked: where nothing else is outside, the class is left out.
+constexpr float TAIL_LEAST = 0x1p-24f;
+template <typename T> constexpr float LOWEST = -0x1.fffffep127f;
+template <> constexpr float LOWEST<__bf16> = -0x1.fep127f;
+template <> constexpr float LOWEST<_Float16> = -65504.0f;
+
+// What q_j, relative to mt, is multiplied with outside the entries.
+__device__ __forceinline__ float outside_factor(const DistillArgs &q, const Mass &e, double dsum, double dtail, float m, float mt, float scale)
 {
+    const double of_row = (e.mass + e.rest) * (mt == m ? 1.0 : exp(((double)mt - (double)m) * q.inv_tau)) / dsum;
+    return (float)((of_row - (e.rest == 0 ? 0.0 : e.rest / dtail)) * (double)scale);
+}
+
+// The divergence, in lane 0 of G: cross = sum p (z - m) / tau; dsum, dtail: sums of the student's exponentials over all
+// actions and over those outside the entries, the latter relative to mt.  Three logarithms, taken by three lanes at once.
+template <int G>
+__device__ __forceinline__ double divergence(const DistillArgs &q, const Mass &e, double cross, double dsum, double dtail, float m, float mt, int lane)
+{
+    const double ratio = e.rest == 0 ? 1.0 : e.rest * dsum / dtail;
     const double l = log(lane == 1 ? dsum : lane == 2 && !(e.rest == 0) ? ratio : lane == 0 && e.norm > 0 ? e.norm : 1.0);
-    const double of_sum = __shfl(l, 1, G), of_ratio = __shfl(l, 2, G);   // of_ratio: of rest dsum / dtail
-    return e.ent - e.mass * l - (cross - e.mass * of_sum) + (e.rest == 0 ? 0.0 : e.rest * of_ratio);
+    const double of_sum = __shfl(l, 1, G), of_ratio = __shfl(l, 2, G);
+    return e.ent - e.mass * l - (cross - e.mass * of_sum) + (e.rest == 0 ? 0.0 : e.rest * (of_ratio + (mt == m ? 0.0 : ((double)m - (double)mt) * q.inv_tau)));
 }
 
 // Small action sets: G lanes of a wave hold a row, E actions and 4 entries a lane, all of it in registers.  MODE 0: loss and
@@ -139,13 +158,13 @@ __global__ __launch_bounds__(256) void k_distill_group(DistillArgs q, float c)
     }
     double p[C];
     Mass e = weigh<G, C>(q, row, index, t, p);
-    if (!e.some || (MODE == 2 ? scale == 0.0f || q.stats[row * 4 + 3] == 0.0f : weight == 0.0f)) {   // nothing of the row counts
+    if (!e.some || (MODE == 2 ? scale == 0.0f || q.stats[row * 4 + 1] == 0.0f : weight == 0.0f)) {   // nothing of the row counts
         if (MODE != 0)
 #pragma unroll
             for (int i = 0; i < E; i++) if (lane + i * G < q.V) gr[lane + i * G] = T(0.0f);
         if (MODE != 2 && lane == 0) {
             q.loss[row] = 0.0f;
-            if (MODE == 0) q.stats[row * 4 + 3] = 0.0f;
+            if (MODE == 0) q.stats[row * 4 + 1] = 0.0f;
         }
         return;
     }
@@ -183,7 +202,7 @@ __global__ __launch_bounds__(256) void k_distill_group(DistillArgs q, float c)
                 }
         }
     }
-    float m;
+    float m, mt;
     double dsum, dtail;
     if (MODE != 2) {
         m = -HUGE_VALF;
@@ -197,30 +216,39 @@ __global__ __launch_bounds__(256) void k_distill_group(DistillArgs q, float c)
             sum += x;
             if (q.lse && !(inside >> i & 1)) tail += x;
         }
-        dsum = group_sum<G>((double)sum), dtail = group_sum<G>((double)tail);
+        dsum = group_sum<G>((double)sum), dtail = group_sum<G>((double)tail), mt = m;
+        if (q.lse && dtail < TAIL_LEAST) {
+            mt = -HUGE_VALF, tail = 0;
+#pragma unroll
+            for (int i = 0; i < E; i++) mt = fmaxf(mt, !(inside >> i & 1) && z[i] > LOWEST<T> ? z[i] : -HUGE_VALF);
+            mt = group_max<G>(mt);
+#pragma unroll
+            for (int i = 0; i < E; i++) tail += !(inside >> i & 1) && z[i] > LOWEST<T> ? expo(z[i] - mt, c) : 0.0f;
+            dtail = group_sum<G>((double)tail);   // 0 where all is masked
+            mt = dtail == 0 ? m : mt;
+        }
         double cross = 0;
 #pragma unroll
         for (int i = 0; i < C; i++)
             if (!(p[i] == 0)) cross += p[i] * (((double)ze[i] - (double)m) * q.inv_tau);
         cross = group_sum<G>(cross);
         if (dtail == 0) e.rest = 0;   // no action outside the entries has anything left
-        const double kl = divergence<G>(e, cross, dsum, e.rest == 0 ? 1.0 : e.rest * dsum / dtail, lane);
+        const double kl = divergence<G>(q, e, cross, dsum, dtail, m, mt, lane);
         if (lane == 0) {
             q.loss[row] = (float)((double)weight * q.tau * q.tau * kl);
-            if (MODE == 0) *(float4 *)(q.stats + row * 4) = make_float4(m, (float)dsum, (float)dtail, 1.0f);
+            if (MODE == 0) *(float4 *)(q.stats + row * 4) = make_float4(m, (float)dsum, (float)dtail, mt);
         }
     } else {
         const float4 st = *(const float4 *)(q.stats + row * 4);
-        m = st.x, dsum = st.y, dtail = st.z;
+        m = st.x, dsum = st.y, dtail = st.z, mt = st.w;
         if (dtail == 0) e.rest = 0;
     }
     if (MODE == 0) return;
-    const double whole = e.mass + e.rest, outside = e.rest == 0 ? whole : whole - e.rest * dsum / dtail, per = (double)scale / dsum;
-    const float f = (float)(outside * per), fi = (float)(whole * per);
+    const float f = outside_factor(q, e, dsum, dtail, m, mt, scale), fi = (float)((e.mass + e.rest) * ((double)scale / dsum));
 #pragma unroll
     for (int i = 0; i < E; i++) {
         const int j = lane + i * G;
-        if (j < q.V && !(inside >> i & 1)) gr[j] = narrow<T>(expo(z[i] - m, c) * f);
+        if (j < q.V && !(inside >> i & 1)) gr[j] = narrow<T>(expo(z[i] - mt, c) * f);
     }
 #pragma unroll
     for (int i = 0; i < C; i++)
@@ -257,7 +285,7 @@ template <> __device__ __forceinline__ unsigned lowest_bits<_Float16>() { return
 // remaining mass: loss 76 us (268 MB, 3.5 TB/s: 4 rows a compute unit, whose first and last steps overlap little), gradient 106 us
 // (536 MB, 5.1 TB/s).  Short rows are bound by the entries' float64 arithmetic: 40000 x 200 in 55 us.
 template <typename T, int THREADS, int NP, int MODE>
-__global__ __launch_bounds__(THREADS, NP == 16 ? 4 : NP ? 6 : 1) void k_distill_row(DistillArgs q, float c)
+__global__ __launch_bounds__(THREADS, NP == 16 ? 4 : NP ? 6 : 8) void k_distill_row(DistillArgs q, float c)
 {
     constexpr int E = 16 / sizeof(T), NW = THREADS / 64, U = NP ? NP : 2;   // packs of a thread on their way at a time
     using P = Pack<T, E>;
@@ -320,7 +348,7 @@ __global__ __launch_bounds__(THREADS, NP == 16 ? 4 : NP ? 6 : 1) void k_distill_
         }
         if (MODE != 2 && tid == 0) {
             q.loss[row] = 0.0f;
-            if (MODE == 0) q.stats[row * 4 + 3] = 0.0f;
+            if (MODE == 0) q.stats[row * 4 + 1] = 0.0f;
         }
     };
 
@@ -332,7 +360,7 @@ __global__ __launch_bounds__(THREADS, NP == 16 ? 4 : NP ? 6 : 1) void k_distill_
 #pragma unroll
             for (int u = 0; u < U; u++) r[u] = load(start + u * THREADS);
     };
-    if (MODE == 2 ? (scale == 0.0f || q.stats[row * 4 + 3] == 0.0f) : weight == 0.0f) {
+    if (MODE == 2 ? (scale == 0.0f || q.stats[row * 4 + 1] == 0.0f) : weight == 0.0f) {
         nothing();
         return;
     }
@@ -384,7 +412,7 @@ __global__ __launch_bounds__(THREADS, NP == 16 ? 4 : NP ? 6 : 1) void k_distill_
         }
         begin();
     } else begin();   // the other waves' first packs are on their way meanwhile
-    float m = -HUGE_VALF, sum = 0, tail = 0;
+    float m = -HUGE_VALF, mt, sum = 0, tail = 0;
     // adds a pack's exponentials to the sums
     auto add = [&](int i, const P &v) {
         float x[E], s = 0;
@@ -472,27 +500,48 @@ __global__ __launch_bounds__(THREADS, NP == 16 ? 4 : NP ? 6 : 1) void k_distill_
         dsum = dtail = 0;
 #pragma unroll
         for (int i = 0; i < NW; i++) dsum += red[0][i], dtail += red[1][i];
+        mt = m;
+        if (bits && !(e.rest == 0) && dtail < TAIL_LEAST) {   // seldom: one more pass, action by action
+            float top = -HUGE_VALF, low = 0;
+            for (int j = tid; j < q.V; j += THREADS) {
+                const float v = widen(z[j]);
+                if (bits[(j + shift) / 32] >> ((j + shift) % 32) & 1 || !(v > LOWEST<T>)) continue;
+                if (v > top) low = top == -HUGE_VALF ? 0.0f : low * expo(top - v, c), top = v;
+                low += expo(v - top, c);
+            }
+            mt = group_max<64>(top);
+            if (lane == 0) red_m[w] = mt;
+            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < NW; i++) mt = fmaxf(mt, red_m[i]);
+            dtail = group_sum<64>(top == -HUGE_VALF ? 0.0 : (double)(low * expo(top - mt, c)));
+            if (lane == 0) red[1][w] = dtail;
+            __syncthreads();
+            dtail = 0;   // and stays so where all is masked
+#pragma unroll
+            for (int i = 0; i < NW; i++) dtail += red[1][i];
+            mt = dtail == 0 ? m : mt;
+        }
         if (dtail == 0) e.rest = 0;   // no action outside the entries has anything left
         if (w == NW - 1) {
             double cross = 0;
             for (int k = lane; k < q.K; k += 64)
                 if (!(ep[k] == 0)) cross += ep[k] * (((double)ez[k] - (double)m) * q.inv_tau);
             cross = group_sum<64>(cross);
-            const double kl = divergence<64>(e, cross, dsum, e.rest == 0 ? 1.0 : e.rest * dsum / dtail, lane);
+            const double kl = divergence<64>(q, e, cross, dsum, dtail, m, mt, lane);
             if (lane == 0) {
                 q.loss[row] = (float)((double)weight * q.tau * q.tau * kl);
-                if (MODE == 0) *(float4 *)(q.stats + row * 4) = make_float4(m, (float)dsum, (float)dtail, 1.0f);
+                if (MODE == 0) *(float4 *)(q.stats + row * 4) = make_float4(m, (float)dsum, (float)dtail, mt);
             }
         }
     } else {
         const float4 st = *(const float4 *)(q.stats + row * 4);
-        m = st.x, dsum = st.y, dtail = st.z;
+        m = st.x, dsum = st.y, dtail = st.z, mt = st.w;
         if (dtail == 0) e.rest = 0;
     }
     if (MODE == 0) return;
     // q_j times what stands outside the entries; the entries themselves are put right behind the barrier
-    const double whole = e.mass + e.rest, outside = e.rest == 0 ? whole : whole - e.rest * dsum / dtail, per = (double)scale / dsum;
-    const float f = (float)(outside * per), fi = (float)(whole * per);
+    const float f = outside_factor(q, e, dsum, dtail, m, mt, scale), fi = (float)((e.mass + e.rest) * ((double)scale / dsum));
     for (int k = tid; k < q.K; k += THREADS) {
         bool other = false;
         for (int i = 0; i < q.K; i++) other |= i != k && ei[i] == ei[k];
@@ -501,7 +550,7 @@ __global__ __launch_bounds__(THREADS, NP == 16 ? 4 : NP ? 6 : 1) void k_distill_
     auto emit = [&](const P &v) {
         P o;
 #pragma unroll
-        for (int k = 0; k < E; k++) o.v[k] = narrow<T>(expo(widen(v.v[k]) - m, c) * f);
+        for (int k = 0; k < E; k++) o.v[k] = narrow<T>(expo(widen(v.v[k]) - mt, c) * f);
         return o;
     };
     if (inner)

@@ -95,8 +95,8 @@ def distillation_loss(logits: torch.Tensor, index: torch.Tensor, teacher: torch.
 
     logits [R, V], index [R, K] (int32 / int64; outside 0..V-1 = absent, the same action twice = summed), teacher [R, K] the
     teacher's logits of those actions (-inf = probability 0).  teacher_lse float32 [R], the log-sum-exp of the teacher's
-    logits / temperature over all actions, keeps its remaining mass as one more class; without it p is renormalised over the
-    entries.  weight float32 [R]: rows of weight 0 and rows without entries have loss and gradient 0 whatever they hold.
+    logits / temperature over all actions, keeps its remaining mass as one more class, all actions outside the entries (left out
+    where all of those are masked at -inf or at the type's lowest value); without it p is renormalised over the entries.  weight float32 [R]: rows of weight 0 and rows without entries have loss and gradient 0 whatever they hold.
     A row whose logits are all -inf, or that holds NaN, gives NaN; an action of probability 0 that the teacher names gives inf."""
     stream = _check_distillation(logits, index, teacher, teacher_lse, weight)
     return _engine.torch_calls().distillation_loss(logits, index, teacher, teacher_lse, weight, float(temperature), stream)
