@@ -453,13 +453,15 @@ int mz_linear_recurrence_workspace(const mz_recurrence *args_h, int32_t backward
 int mz_linear_recurrence(const mz_recurrence *args_h, void *stream);
 int mz_linear_recurrence_backward(const mz_recurrence *args_h, void *stream);
 
-/* Distillation of a policy from a teacher's top logits: loss[r] = weight[r] * temperature^2 * KL(p || q), q =
- * softmax(logits / temperature) over the V actions; p = softmax(teacher / temperature) over the K entries, or, with lse
+/* Distillation of a policy from a teacher's top logits: loss[r] = weight[r] * temperature^2 * sum_k p_k (log p_k -
+ * log q(index_k)), the divergence KL(p || q) where no action is named twice; q = softmax(logits / temperature) over the V actions; p = softmax(teacher / temperature) over the K entries, or, with lse
  * (log-sum-exp of the teacher's logits / temperature over all actions), p = exp(teacher / temperature - lse) and one more
  * class of all actions outside the entries (left out where all of those are masked: logits of -inf, or of the type's lowest
  * value and next to nothing).  The soft cross-entropy the trainer takes over whole rows (trainer.py:119-122), for targets that
  * name few actions.
- * Entries whose index lies outside 0..V-1 are absent; an action named twice gets the sum.  Rows without entries and
+ * Entries whose index lies outside 0..V-1 are absent.  Entries that name one action each have their own term: the gradient is
+ * that of the sum of their p, the loss is KL(p || q) of those sums less the entropy of the choice between such entries, sum_k p_k
+ * log(sum / p_k), which the student cannot change (two equal entries alone: log 2 less, so it may be negative).  Rows without entries and
  * rows of weight 0 have loss and gradient 0 whatever their logits hold.
  * mz_distill_loss: loss and stats.  mz_distill_grad: grad = grad_loss[r] * d loss[r] / d logits from those stats.
  * mz_distill_loss_grad: loss and grad (grad_loss taken as 1) with the logits read once. */

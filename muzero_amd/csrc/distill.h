@@ -4,7 +4,8 @@
 //   p_k = softmax(t / tau) over the entries, or exp(t_k / tau - lse) where the teacher's log-sum-exp over all actions is
 //         given; rest = 1 - sum p is then one more class: everything outside the entries
 //   q   = softmax(z / tau)
-//   loss = w tau^2 [ sum_k p_k (log p_k - log q_k) + rest (log rest - log qrest) ]
+//   loss = w tau^2 [ sum_k p_k (log p_k - log q_k) + rest (log rest - log qrest) ],  k over the entries: those of one action have
+//         a term each, which is the divergence of their sum less the entropy of the choice between them, no matter of q
 //   dz_j = w tau [ q_j (sum p + rest) - p_j ]  inside the entries,  w tau q_j [ sum p + rest - rest / qrest ]  outside
 //
 // Sums of exponentials run in float32 per thread and are joined in float64; what concerns the few entries is float64

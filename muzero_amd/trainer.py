@@ -89,12 +89,15 @@ def _check_distillation(logits, index, teacher, lse, weight) -> int:
 
 def distillation_loss(logits: torch.Tensor, index: torch.Tensor, teacher: torch.Tensor, teacher_lse: Optional[torch.Tensor] = None,
                       temperature: float = 1.0, weight: Optional[torch.Tensor] = None) -> torch.Tensor:
-    """Per-row distillation loss float32 [R], differentiable in logits: weight * temperature^2 * KL(p || q) with
-    q = softmax(logits / temperature) over all V actions and p the teacher's distribution over its K entries - what
-    `soft_cross_entropy` takes over whole rows, for targets that name few actions out of many.
+    """Per-row distillation loss float32 [R], differentiable in logits: weight * temperature^2 * sum_k p_k (log p_k -
+    log q(index_k)), the divergence KL(p || q) where no action is named twice, with q = softmax(logits / temperature) over all V
+    actions and p the teacher's distribution over its K entries - what `soft_cross_entropy` takes over whole rows, for targets
+    that name few actions out of many.
 
-    logits [R, V], index [R, K] (int32 / int64; outside 0..V-1 = absent, the same action twice = summed), teacher [R, K] the
-    teacher's logits of those actions (-inf = probability 0).  teacher_lse float32 [R], the log-sum-exp of the teacher's
+    logits [R, V], index [R, K] (int32 / int64; outside 0..V-1 = absent), teacher [R, K] the teacher's logits of those actions
+    (-inf = probability 0).  Entries that name the same action have a term each: the gradient is that of their summed p, the loss
+    is KL(p || q) of the sums less the entropy of the choice between them, a constant of the teacher (merge such entries with
+    `logsumexp` beforehand for the divergence itself).  teacher_lse float32 [R], the log-sum-exp of the teacher's
     logits / temperature over all actions, keeps its remaining mass as one more class, all actions outside the entries (left out
     where all of those are masked at -inf or at the type's lowest value); without it p is renormalised over the entries.  weight float32 [R]: rows of weight 0 and rows without entries have loss and gradient 0 whatever they hold.
     A row whose logits are all -inf, or that holds NaN, gives NaN; an action of probability 0 that the teacher names gives inf."""
