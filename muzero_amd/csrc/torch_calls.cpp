@@ -4,6 +4,7 @@
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/extension.h>
 
+#include <initializer_list>
 #include <string>
 #include <tuple>
 #include <vector>
@@ -45,6 +46,14 @@ static int type_of(const Tensor &t)
 }
 
 static void *ptr(const Tensor &t) { return t.defined() ? t.data_ptr() : nullptr; }
+
+// What the kernels compute is no torch operation, so a tangent would be dropped: an error.
+static void refuse(const char *fn, std::initializer_list<Tensor> inputs)
+{
+    for (const Tensor &t : inputs)
+        TORCH_CHECK_NOT_IMPLEMENTED(!t.defined() || !t._fw_grad(0).defined(), fn, ": no forward-mode derivatives");
+}
+static Tensor given(const std::optional<Tensor> &t) { return t.value_or(Tensor()); }
 
 // A gradient taken with create_graph: the operators are differentiable once, and a second time is an error, not a zero.
 static variable_list once(variable_list grads)
@@ -128,7 +137,7 @@ struct Recurrence : torch::autograd::Function<Recurrence> {
     static variable_list forward(AutogradContext *ctx, const Tensor &gate, const Tensor &x, const std::optional<Tensor> &first, bool reverse,
                                  int64_t stream)
     {
-        const Tensor state = first.value_or(Tensor());
+        const Tensor state = given(first);
         auto [y, last, fine] = recurrence_forward(gate, x, state, reverse, gate.requires_grad(), stream);
         ctx->set_materialize_grads(false);
         ctx->saved_data["reverse"] = reverse;
@@ -168,6 +177,7 @@ struct Recurrence : torch::autograd::Function<Recurrence> {
 
 static std::tuple<Tensor, Tensor> linear_recurrence(const Tensor &gate, const Tensor &x, const std::optional<Tensor> &state, bool reverse, int64_t stream)
 {
+    refuse("linear_recurrence", {gate, x, given(state)});
     const Tensor s = state ? state->contiguous() : Tensor();
     if (at::GradMode::is_enabled() && (gate.requires_grad() || x.requires_grad() || (s.defined() && s.requires_grad()))) {
         auto out = Recurrence::apply(gate, x, s.defined() ? std::optional<Tensor>(s) : std::nullopt, reverse, stream);
@@ -197,7 +207,7 @@ struct Distillation : torch::autograd::Function<Distillation> {
     static Tensor forward(AutogradContext *ctx, const Tensor &logits, const Tensor &index, const Tensor &teacher,
                           const std::optional<Tensor> &lse, const std::optional<Tensor> &weight, double temperature, int64_t stream)
     {
-        variable_list t{logits.detach(), index, teacher.detach(), lse.value_or(Tensor()), weight.value_or(Tensor())};
+        variable_list t{logits.detach(), index, teacher.detach(), given(lse), given(weight)};
         mz_distill a = distill_args(t, temperature);
         const auto f32 = logits.options().dtype(at::kFloat);
         Tensor loss = at::empty({logits.size(0)}, f32), stats = at::empty({logits.size(0), 4}, f32);
@@ -230,6 +240,7 @@ struct Distillation : torch::autograd::Function<Distillation> {
 static Tensor distillation_loss(const Tensor &logits, const Tensor &index, const Tensor &teacher, const std::optional<Tensor> &lse,
                                 const std::optional<Tensor> &weight, double temperature, int64_t stream)
 {
+    refuse("distillation_loss", {logits, index, teacher, given(lse), given(weight)});
     auto plain = [](const std::optional<Tensor> &t) { return t ? std::optional<Tensor>(t->detach()) : std::nullopt; };
     return Distillation::apply(logits, index, teacher.detach(), plain(lse), plain(weight), temperature, stream);
 }
@@ -238,8 +249,9 @@ static std::tuple<Tensor, Tensor> distillation_loss_grad(const Tensor &logits, c
                                                          const std::optional<Tensor> &lse, const std::optional<Tensor> &weight,
                                                          double temperature, int64_t stream)
 {
+    refuse("distillation_loss_grad", {logits, index, teacher, given(lse), given(weight)});
     at::AutoGradMode off(false);
-    variable_list t{logits, index, teacher, lse.value_or(Tensor()), weight.value_or(Tensor())};
+    variable_list t{logits, index, teacher, given(lse), given(weight)};
     mz_distill a = distill_args(t, temperature);
     Tensor loss = at::empty({logits.size(0)}, logits.options().dtype(at::kFloat)), grad = at::empty(logits.sizes(), logits.options());
     a.loss = loss.data_ptr<float>(), a.grad = grad.data_ptr();
@@ -253,6 +265,7 @@ static std::tuple<Tensor, Tensor> distillation_loss_grad(const Tensor &logits, c
 static std::tuple<Tensor, Tensor> verify_drafts(Tensor tokens, std::optional<Tensor> draft, Tensor target, Tensor u_accept, Tensor u_sample,
                                                 std::optional<Tensor> lengths, int64_t stream)
 {
+    refuse("verify_drafts", {tokens, given(draft), target, u_accept, u_sample, given(lengths)});
     at::AutoGradMode off(false);
     const int64_t B = tokens.size(0), K = tokens.size(1), V = target.size(2);
     Tensor accepted = at::empty({B}, target.options().dtype(at::kInt)), out = at::empty({B, K + 1}, tokens.options());
