@@ -1,7 +1,9 @@
 // The tensor operators as torch sees them: outputs allocated, layouts lined up, gradients recorded as native autograd nodes, so
 // that a call costs little more than its launch.  Host code only: the C entries' addresses (include/muzero_amd.h) and the raw
 // stream come from Python, which has checked types, shapes and devices; a backward pass runs on its forward pass's stream.
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/extension.h>
 
 #include <initializer_list>
@@ -47,11 +49,15 @@ static int type_of(const Tensor &t)
 
 static void *ptr(const Tensor &t) { return t.defined() ? t.data_ptr() : nullptr; }
 
-// What the kernels compute is no torch operation, so a tangent would be dropped: an error.
+// What the kernels compute is no torch operation, so a tangent would be dropped and a trace would hold outputs that nothing
+// fills: both are errors.
 static void refuse(const char *fn, std::initializer_list<Tensor> inputs)
 {
     for (const Tensor &t : inputs)
         TORCH_CHECK_NOT_IMPLEMENTED(!t.defined() || !t._fw_grad(0).defined(), fn, ": no forward-mode derivatives");
+    using c10::impl::TorchDispatchModeTLS;
+    TORCH_CHECK_NOT_IMPLEMENTED(!torch::jit::tracer::isTracing() && !TorchDispatchModeTLS::get_mode(c10::impl::TorchDispatchModeKey::PROXY), fn,
+                                " cannot be traced");
 }
 static Tensor given(const std::optional<Tensor> &t) { return t.value_or(Tensor()); }
 

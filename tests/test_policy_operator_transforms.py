@@ -1,8 +1,9 @@
-"""Transformations of torch that go round the tensor operators' native calls must raise: a tangent that is dropped
-would be silent.  CPU: at the native calls, which refuse before anything is launched; GPU: at the public ones."""
+"""Transformations of torch that go round the tensor operators' native calls must raise: a tangent that is dropped and a trace
+that fills nothing would be silent.  CPU: at the native calls, which refuse before anything is launched; GPU: at the public ones."""
 import pytest
 import torch
 import torch.autograd.forward_ad as fwad
+from torch.fx.experimental.proxy_tensor import make_fx
 
 
 def recurrence_args(device):
@@ -47,6 +48,10 @@ def check(calls, device):
                     call(*dual)
                 with torch.no_grad(), pytest.raises(NotImplementedError, match='forward-mode'):
                     call(*dual)
+        with pytest.raises(NotImplementedError, match='traced'):
+            torch.jit.trace(call, args, check_trace=False)
+        with pytest.raises(NotImplementedError, match='traced'):
+            make_fx(call, tracing_mode='real')(*args)
 
 
 def test_native_calls():
