@@ -13,6 +13,13 @@
 
 using namespace mz;
 
+// A launch takes fewer than 2^32 threads: larger calls are launched in slices of at most so many blocks (of 1024 threads at most).
+constexpr long long SLICE = 1 << 20;
+constexpr long long MOST_THREADS = (1ll << 32) - 1;
+
+static const char *ahead(const void *p, long long bytes) { return p ? (const char *)p + bytes : nullptr; }
+static char *ahead(void *p, long long bytes) { return p ? (char *)p + bytes : nullptr; }
+
 static size_t size_of(int type) { return type == MZ_F64 ? 8 : type == MZ_F32 ? 4 : 2; }
 
 // ------------------------------------------------------------------------------------------------ recurrence
@@ -55,7 +62,8 @@ static RecurrencePlan plan_recurrence(const mz_recurrence *a, bool backward)
     if (a->D == 1) p.channels = false;
     if (!p.channels) {
         const long long links = (a->T + ROW_LINK - 1) / ROW_LINK;
-        if ((long long)a->B * a->D < REC_FEW_ROWS && links >= REC_LEAST_ROW_LINKS && links < INT32_MAX / REC_FEW_ROWS) p.links = (int)links;
+        const long long rows = (long long)a->B * a->D;
+        if (rows < REC_FEW_ROWS && links >= REC_LEAST_ROW_LINKS && links <= MOST_THREADS / 1024 / rows) p.links = (int)links;
         return p;
     }
     auto fits = [&](int n) { return a->D % n == 0 && low % (uint64_t)(n * size) == 0; };
@@ -72,7 +80,8 @@ static RecurrencePlan plan_recurrence(const mz_recurrence *a, bool backward)
     p.lanes = tiles_of(64) >= REC_MANY_TILES ? 64 : 32;
     p.strands = (int)std::min<long long>(REC_THREADS / p.lanes, std::max<long long>(2, (a->T + REC_LENGTH - 1) / REC_LENGTH));
     const long long links = (a->T + CHAIN_ROWS(size, backward) - 1) / CHAIN_ROWS(size, backward);
-    if (a->T > 256 && tiles_of(32) < (backward ? REC_FEW_TILES_BACKWARD : REC_FEW_TILES) && links >= REC_LEAST_LINKS && links * tiles_of(64) < INT32_MAX) p.links = (int)links;
+    if (a->T > 256 && tiles_of(32) < (backward ? REC_FEW_TILES_BACKWARD : REC_FEW_TILES) && links >= REC_LEAST_LINKS &&
+        links <= MOST_THREADS / (64 * CHAIN_WAVES(size, backward)) / tiles_of(64)) p.links = (int)links;
     return p;
 }
 
@@ -139,6 +148,25 @@ template <typename T, bool BWD> static void launch_recurrence(const RecurrencePl
     else launch_channels<T, 1, BWD>(p, q, st);
 }
 
+// q in slices of sequences, and one sequence in slices of channels, where it is more than one launch can take.
+template <typename T, bool BWD> static void launch_slices(const RecurrencePlan &p, const RecurrenceArgs &q, hipStream_t st)
+{
+    // channels of a block; a chain is one launch by its plan, a thread of k_recurrence_short serves a channel at least
+    const long long wide = p.channels ? (long long)p.lanes * p.vec : 1, blocks = (q.D + wide - 1) / wide;
+    if (p.links || p.brief || blocks * q.B <= SLICE) return launch_recurrence<T, BWD>(p, q, st);
+    const int sequences = (int)std::max(1ll, SLICE / blocks), channels = (int)std::min<long long>(q.D, SLICE * wide);
+    for (int b = 0; b < q.B; b += sequences)
+        for (int d = 0; d < q.D; d += channels) {
+            RecurrenceArgs s = q;
+            s.B = std::min(sequences, q.B - b), s.D = std::min(channels, q.D - d);
+            for (RecurrenceArgs::View *v : {&s.a, &s.x, &s.y, &s.out, &s.da}) v->p = ahead(v->p, (b * v->sb + d * v->sd) * (long long)sizeof(T));
+            s.fine.p = ahead(s.fine.p, b * s.fine.sb + d * s.fine.sd);
+            const long long state = ((long long)b * q.D + d) * (long long)sizeof(acc_t<T>);
+            s.first = ahead(s.first, state), s.state0 = ahead(s.state0, state), s.last = ahead(s.last, state);
+            launch_recurrence<T, BWD>(p, s, st);
+        }
+}
+
 static int check_recurrence(const mz_recurrence *a, bool backward, const char *fn)
 {
     if (!a) return api_fail(MZ_ERR_ARG, std::string(fn) + ": null argument");
@@ -175,10 +203,10 @@ template <bool BWD> static int run_recurrence(const mz_recurrence *a, void *stre
     q.first = BWD ? a->grad_last : a->state, q.last = BWD ? a->out_state : a->last;
     hipStream_t st = (hipStream_t)stream;
     switch (a->type) {
-    case MZ_F32: launch_recurrence<float, BWD>(p, q, st); break;
-    case MZ_BF16: launch_recurrence<__bf16, BWD>(p, q, st); break;
-    case MZ_F16: launch_recurrence<_Float16, BWD>(p, q, st); break;
-    default: launch_recurrence<double, BWD>(p, q, st);
+    case MZ_F32: launch_slices<float, BWD>(p, q, st); break;
+    case MZ_BF16: launch_slices<__bf16, BWD>(p, q, st); break;
+    case MZ_F16: launch_slices<_Float16, BWD>(p, q, st); break;
+    default: launch_slices<double, BWD>(p, q, st);
     }
     return api_launch_status(fn);
 }
@@ -238,6 +266,20 @@ template <typename T, int MODE> static void launch_distill(const DistillArgs &q,
     else launch_row<T, MODE == 0 ? 512 : 1024, 0, MODE>(q, c, st);
 }
 
+template <typename T, int MODE> static void launch_distill_slices(const DistillArgs &q, float c, hipStream_t st)
+{
+    for (long long r = 0; r < q.R; r += SLICE) {
+        DistillArgs s = q;
+        const long long k = r * q.K;
+        s.R = (int)std::min(SLICE, q.R - r);
+        s.logits = ahead(q.logits, r * q.ld * (long long)sizeof(T)), s.grad = ahead(q.grad, r * q.V * (long long)sizeof(T));
+        s.index = ahead(q.index, k * (q.index64 ? 8 : 4)), s.teacher = ahead(q.teacher, k * (long long)size_of(q.teacher_type));
+        s.lse = (const float *)ahead(q.lse, r * 4), s.weight = (const float *)ahead(q.weight, r * 4), s.up = (const float *)ahead(q.up, r * 4);
+        s.loss = (float *)ahead(q.loss, r * 4), s.stats = (float *)ahead(q.stats, r * 16);
+        launch_distill<T, MODE>(s, c, st);
+    }
+}
+
 template <int MODE> static int run_distill(const mz_distill *a, void *stream, const char *fn)
 {
     (void)hipGetLastError();
@@ -258,9 +300,9 @@ template <int MODE> static int run_distill(const mz_distill *a, void *stream, co
     const float c = (float)(1.4426950408889634074 / (double)a->temperature);   // log2(e) / temperature
     hipStream_t st = (hipStream_t)stream;
     switch (a->type) {
-    case MZ_F32: launch_distill<float, MODE>(q, c, st); break;
-    case MZ_BF16: launch_distill<__bf16, MODE>(q, c, st); break;
-    default: launch_distill<_Float16, MODE>(q, c, st);
+    case MZ_F32: launch_distill_slices<float, MODE>(q, c, st); break;
+    case MZ_BF16: launch_distill_slices<__bf16, MODE>(q, c, st); break;
+    default: launch_distill_slices<_Float16, MODE>(q, c, st);
     }
     return api_launch_status(fn);
 }
@@ -287,6 +329,19 @@ template <typename T> static void launch_verify(const VerifyArgs &q, hipStream_t
     hipLaunchKernelGGL((k_verify<T>), dim3((unsigned)q.B), dim3(64 * std::min(stretches, 16)), 8 * (size_t)stretches, st, q);
 }
 
+template <typename T> static void launch_verify_slices(const VerifyArgs &q, hipStream_t st)
+{
+    const long long token = q.token64 ? 8 : 4, size = (long long)sizeof(T);
+    for (long long b = 0; b < q.B; b += SLICE) {
+        VerifyArgs s = q;
+        s.B = (int)std::min(SLICE, q.B - b);
+        s.tokens = ahead(q.tokens, b * q.K * token), s.draft = ahead(q.draft, b * q.draft_b * size), s.target = ahead(q.target, b * q.target_b * size);
+        s.u_accept = (const double *)ahead(q.u_accept, b * q.K * 8), s.u_sample = q.u_sample + b, s.lengths = (const int *)ahead(q.lengths, b * 4);
+        s.accepted = q.accepted + b, s.out = ahead(q.out, b * (q.K + 1ll) * token);
+        launch_verify<T>(s, st);
+    }
+}
+
 extern "C" int mz_verify_drafts(const mz_verify *a, void *stream)
 {
     const char *fn = "mz_verify_drafts";
@@ -304,10 +359,10 @@ extern "C" int mz_verify_drafts(const mz_verify *a, void *stream)
     q.B = a->B, q.K = a->K, q.V = a->V, q.token64 = a->token64;
     hipStream_t st = (hipStream_t)stream;
     switch (a->type) {
-    case MZ_F32: launch_verify<float>(q, st); break;
-    case MZ_BF16: launch_verify<__bf16>(q, st); break;
-    case MZ_F16: launch_verify<_Float16>(q, st); break;
-    default: launch_verify<double>(q, st);
+    case MZ_F32: launch_verify_slices<float>(q, st); break;
+    case MZ_BF16: launch_verify_slices<__bf16>(q, st); break;
+    case MZ_F16: launch_verify_slices<_Float16>(q, st); break;
+    default: launch_verify_slices<double>(q, st);
     }
     return api_launch_status(fn);
 }

@@ -31,8 +31,9 @@ def public():
     from muzero_amd.drafts import verify_drafts
     from muzero_amd.targets import linear_recurrence
     from muzero_amd.trainer import distillation_loss, distillation_loss_grad
-    return [(linear_recurrence, recurrence_args), (lambda z, i, t, e, w: distillation_loss(z, i, t, e, weight=w), distill_args),
-            (lambda z, i, t, e, w: distillation_loss_grad(z, i, t, e, weight=w), distill_args), (verify_drafts, verify_args)]
+    return [(lambda a, x, s: linear_recurrence(a, x, s), recurrence_args), (lambda z, i, t, e, w: distillation_loss(z, i, t, e, weight=w), distill_args),
+            (lambda z, i, t, e, w: distillation_loss_grad(z, i, t, e, weight=w), distill_args),
+            (lambda *a: verify_drafts(*a), verify_args)]
 
 
 def check(calls, device):
