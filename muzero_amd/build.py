@@ -53,13 +53,6 @@ def source_fingerprint() -> str:
     return h.hexdigest()[:16]
 
 
-def needs_build(lib: str = LIB) -> bool:
-    if not os.path.exists(lib):
-        return True
-    t = os.path.getmtime(lib)
-    return any(os.path.getmtime(os.path.join(CSRC, f)) > t for f in SOURCES + HEADERS)
-
-
 # headers a translation unit does NOT include (everything else counts as a dependency)
 _TREE_ONLY = {'search_net.h', 'search_reg.h', 'env_step.h', 'targets.h', 'api.h'} | _POLICY
 NOT_INCLUDED = {'engine.hip': {'net_mfma.h', 'search_cached.h', 'search_chain.h', 'cached_launch.h'} | _POLICY,
@@ -71,32 +64,64 @@ NOT_INCLUDED = {'engine.hip': {'net_mfma.h', 'search_cached.h', 'search_chain.h'
                 'cached_kernels_c.hip': _TREE_ONLY | {'search_chain.h'}}
 
 
-def _stale(src: str, obj: str) -> bool:
-    if not os.path.exists(obj):
+def _object(src: str, defines=()) -> str:
+    tag = '_'.join(defines).replace('=', '')
+    return os.path.join(OBJ_DIR, src.replace('.hip', f'{"_" + tag if tag else ""}.o'))
+
+
+def _command(src: str, defines=()) -> list:
+    return [os.environ.get('HIPCC', '/opt/rocm/bin/hipcc'), *FLAGS, *OPT.get(src, OPT_DEFAULT).split(), *[f'-D{x}' for x in defines], '-c',
+            os.path.join(CSRC, src), '-o', _object(src, defines)]
+
+
+def _recipe(target: str) -> str:
+    """Where the text of the command that built `target` is kept: one built by another command is as stale as one built from
+    other sources."""
+    return os.path.join(OBJ_DIR, os.path.basename(target) + '.command')
+
+
+def _newer_or_other(target: str, deps, command) -> bool:
+    try:
+        t = os.path.getmtime(target)
+        with open(_recipe(target)) as fh:
+            return fh.read() != repr(command) or any(os.path.getmtime(f) > t for f in deps)
+    except FileNotFoundError:
         return True
-    t = os.path.getmtime(obj)
+
+
+def _run(target: str, command) -> None:
+    os.makedirs(OBJ_DIR, exist_ok=True)
+    if os.path.exists(_recipe(target)):
+        os.remove(_recipe(target))
+    subprocess.check_call(command)
+    with open(_recipe(target), 'w') as fh:
+        fh.write(repr(command))
+
+
+def _stale(src: str, defines=()) -> bool:
     deps = [src] + [h for h in HEADERS if os.path.basename(h) not in NOT_INCLUDED.get(src, set())]
-    return any(os.path.getmtime(os.path.join(CSRC, f)) > t for f in deps)
+    return _newer_or_other(_object(src, defines), [os.path.join(CSRC, f) for f in deps], _command(src, defines))
 
 
 def build_torch_calls(force: bool = False) -> str:
     """Host code only (the host compiler, torch's headers and libraries; no GPU headers)."""
-    deps = [TORCH_SOURCE, os.path.join(HERE, '..', 'include', 'muzero_amd.h')]
-    if force or not os.path.exists(TORCH_LIB) or any(os.path.getmtime(f) > os.path.getmtime(TORCH_LIB) for f in deps):
-        import torch
-        root = os.path.dirname(torch.__file__)
-        include = [os.path.join(root, 'include'), os.path.join(root, 'include', 'torch', 'csrc', 'api', 'include'),
-                   sysconfig.get_paths()['include']]
-        libs = os.path.join(root, 'lib')
-        subprocess.check_call([os.environ.get('CXX', 'g++'), '-O2', '-std=c++17', '-fPIC', '-shared', '-DTORCH_EXTENSION_NAME=_torch_calls',
-                               '-DTORCH_API_INCLUDE_EXTENSION_H', f'-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}',
-                               *[f'-I{i}' for i in include], TORCH_SOURCE, '-o', TORCH_LIB, f'-L{libs}', f'-Wl,-rpath,{libs}', '-lc10',
-                               '-ltorch_cpu', '-ltorch_python'])
+    import torch
+    root = os.path.dirname(torch.__file__)
+    include = [os.path.join(root, 'include'), os.path.join(root, 'include', 'torch', 'csrc', 'api', 'include'),
+               sysconfig.get_paths()['include']]
+    libs = os.path.join(root, 'lib')
+    # the version stands in the command: a binding built against another torch is built again (and refused where it is loaded)
+    command = [os.environ.get('CXX', 'g++'), '-O2', '-std=c++17', '-fPIC', '-shared', '-DTORCH_EXTENSION_NAME=_torch_calls',
+               '-DTORCH_API_INCLUDE_EXTENSION_H', f'-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}',
+               f'-DBUILT_FOR_TORCH="{torch.__version__}"', *[f'-I{i}' for i in include], TORCH_SOURCE, '-o', TORCH_LIB, f'-L{libs}',
+               f'-Wl,-rpath,{libs}', '-lc10', '-ltorch_cpu', '-ltorch_python']
+    if force or _newer_or_other(TORCH_LIB, [TORCH_SOURCE, os.path.join(HERE, '..', 'include', 'muzero_amd.h')], command):
+        _run(TORCH_LIB, command)
     return TORCH_LIB
 
 
 def build(force: bool = False, defines=(), lib: str = LIB) -> str:
-    """Compiles the translation units that changed (all of them with `force`), in parallel, and links the shared
+    """Compiles the translation units whose sources or command changed (all of them with `force`), in parallel, and links the shared
     library.  `defines`: extra -D flags (the diagnostic build with phase stamps uses MZ_STAMPS and another `lib`)."""
     with ThreadPoolExecutor(1) as beside:
         binding = beside.submit(build_torch_calls, force) if lib == LIB else None
@@ -107,20 +132,14 @@ def build(force: bool = False, defines=(), lib: str = LIB) -> str:
 
 
 def _build_library(force, defines, lib) -> None:
-    if force or needs_build(lib):
-        hipcc = os.environ.get('HIPCC', '/opt/rocm/bin/hipcc')
-        os.makedirs(OBJ_DIR, exist_ok=True)
-        tag = '_'.join(defines).replace('=', '')
-        objs = [os.path.join(OBJ_DIR, s.replace('.hip', f'{"_" + tag if tag else ""}.o')) for s in SOURCES]
-        todo = [(s, o) for s, o in zip(SOURCES, objs) if force or _stale(s, o)]
-
-        def compile_one(pair):
-            src, obj = pair
-            subprocess.check_call([hipcc, *FLAGS, *OPT.get(src, OPT_DEFAULT).split(), *[f'-D{x}' for x in defines], '-c',
-                                   os.path.join(CSRC, src), '-o', obj])
-        with ThreadPoolExecutor(max(len(todo), 1)) as pool:
-            list(pool.map(compile_one, todo))
-        subprocess.check_call([hipcc, '--offload-arch=gfx950', '-shared', '-fPIC', *objs, '-o', lib])
+    todo = [s for s in SOURCES if force or _stale(s, defines)]
+    if todo:
+        with ThreadPoolExecutor(len(todo)) as pool:
+            list(pool.map(lambda s: _run(_object(s, defines), _command(s, defines)), todo))
+    objs = [_object(s, defines) for s in SOURCES]
+    link = [os.environ.get('HIPCC', '/opt/rocm/bin/hipcc'), '--offload-arch=gfx950', '-shared', '-fPIC', *objs, '-o', lib]
+    if todo or _newer_or_other(lib, objs, link):
+        _run(lib, link)
 
 
 if __name__ == '__main__':

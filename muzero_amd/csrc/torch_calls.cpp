@@ -295,6 +295,7 @@ static std::tuple<Tensor, Tensor> verify_drafts(Tensor tokens, std::optional<Ten
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m)
 {
+    m.attr("built_for") = BUILT_FOR_TORCH;
     m.def("bind", &bind);
     m.def("linear_recurrence", &linear_recurrence);
     m.def("distillation_loss", &distillation_loss);

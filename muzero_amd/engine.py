@@ -244,6 +244,9 @@ def torch_calls():
         spec = importlib.util.spec_from_file_location('_torch_calls', path)
         module = importlib.util.module_from_spec(spec)
         spec.loader.exec_module(module)
+        if module.built_for != torch.__version__:
+            raise EngineError(f'{path} was built for torch {module.built_for}, this is {torch.__version__}: build it again with '
+                              '`python -m muzero_amd.build`.')
         module.bind([C.cast(getattr(L, name), C.c_void_p).value for name in (
             'mz_linear_recurrence', 'mz_linear_recurrence_backward', 'mz_linear_recurrence_workspace', 'mz_distill_loss', 'mz_distill_grad',
             'mz_distill_loss_grad', 'mz_verify_drafts', 'mz_last_error')])
