@@ -426,7 +426,8 @@ typedef struct mz_strided {
 /* Gated linear recurrence along T, out[t] = gate[t] * out[t-1] + x[t] (reverse: out[t] = gate[t] * out[t+1] + x[t]), the
  * sum behind discounted returns and traces (games/game.py:205-236 sums one of them term by term).  All tensors of one
  * element type; states [B][D] contiguous, float32 (float64 for MZ_F64), as is the arithmetic: one rounding per output.
- * Runs of positions are composed through products of their gates, which must not overflow (|gate| <= 1 cannot).
+ * Runs of positions are composed through products of their gates, which must not overflow (|gate| <= 1 cannot); what follows
+ * an infinite output of its row is infinite or NaN.
  * mz_linear_recurrence: gate, x -> out; state = what precedes the first position (NULL: 0), last = the state behind the
  * last position (may be NULL).
  * mz_linear_recurrence_backward: gate as before, x = gradient of out -> out = gradient of x; with y = the outputs,
@@ -510,7 +511,7 @@ typedef struct mz_verify {
 } mz_verify;
 int mz_verify_drafts(const mz_verify *args_h, void *stream);
 
-/* Library/ABI version. */
+/* Library/ABI version.  2: mz_recurrence ends in `fine`. */
 int mz_version(void);
 
 #ifdef __cplusplus

@@ -130,8 +130,9 @@ __device__ __forceinline__ double divergence(const DistillArgs &q, const Mass &e
 
 // Small action sets: G lanes of a wave hold a row, E actions and 4 entries a lane, all of it in registers.  MODE 0: loss and
 // statistics, 1: loss and gradient, 2: gradient from the statistics of an earlier loss pass.  98304 rows of 9 float32, 4
-// entries: 8.3 us for the loss, 7.4 for the gradient - two to three times their bytes, bound by the float64 arithmetic of the
-// entries (one exponential and one logarithm a lane).
+// entries: 8.4 us for the loss, 7.8 for the gradient - two to three times their bytes.  A wave runs 470 (350) vector instructions,
+// most of them for the entries in float64, the vector units issue in a sixth of their cycles and waves wait for half of theirs:
+// index, logit, exponential, sums over lanes and logarithm each need the one before.  40000 rows of 64, 20 entries: 21 us.
 template <typename T, int G, int E, int MODE>
 __global__ __launch_bounds__(256) void k_distill_group(DistillArgs q, float c)
 {
@@ -284,7 +285,8 @@ template <> __device__ __forceinline__ unsigned lowest_bits<_Float16>() { return
 // between the two (NP > 0) and reads wider ones again.
 // 4096 x 32000 bfloat16, 32 entries, loss and gradient: 116 us (524 MB, 4.5 TB/s; a copy 5.1).  1023 x 131071, 64 entries and the
 // remaining mass: loss 76 us (268 MB, 3.5 TB/s: 4 rows a compute unit, whose first and last steps overlap little), gradient 106 us
-// (536 MB, 5.1 TB/s).  Short rows are bound by the entries' float64 arithmetic: 40000 x 200 in 55 us.
+// (536 MB, 5.1 TB/s).  Short rows are bound by the same chain as above, one row at a time: 40000 x 200 float32, 20 entries in 57 us,
+// 790 vector instructions a wave and units that issue in a quarter of their cycles.
 template <typename T, int THREADS, int NP, int MODE>
 __global__ __launch_bounds__(THREADS, NP == 16 ? 4 : NP ? 6 : 8) void k_distill_row(DistillArgs q, float c)
 {

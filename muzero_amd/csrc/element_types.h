@@ -15,7 +15,7 @@ template <typename T> __device__ __forceinline__ acc_t<T> widen(T v) { return (a
 template <typename T> __device__ __forceinline__ T narrow(acc_t<T> v) { return (T)v; }
 
 // What a rounding to 16 bits lost, in 8 more bits: the distance of the float32 pattern from that of the rounded value (patterns
-// of one sign are ordered like their values, across exponents too) in steps of 2^FINE_SHIFT, held in byte FINE_BYTE of what
+// of one sign are ordered like their values, across exponents too) in steps of 2^FINE_SHIFT, held in byte 1 of what
 // fine_of() returns.  refined() is then within one such step of the float32 value, 2^-15 of it (bfloat16) or 2^-18 (float16).
 // A bfloat16 has float32's exponents: half a step of its own is 2^15 everywhere, what rounds to infinity comes back finite, and
 // adding up to 2^15 to a quiet NaN leaves one.  A float16 among its subnormal numbers is off by more than fits and is never

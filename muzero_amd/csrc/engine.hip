@@ -332,7 +332,7 @@ extern "C" int mz_legacy_gumbel(uint32_t *mt_key, int32_t *mt_pos, int64_t n, do
 }
 
 extern "C" const char *mz_last_error(void) { return g_err.c_str(); }
-extern "C" int mz_version(void) { return 1; }
+extern "C" int mz_version(void) { return 2; }
 
 template <typename T>
 static int dev_alloc(mz_ctx *c, T **p, size_t n)

@@ -28,13 +28,13 @@ static size_t size_of(int type) { return type == MZ_F64 ? 8 : type == MZ_F32 ? 4
 // - REC_LENGTH, positions a strand of k_recurrence_channels holds in registers: 8 x 4096 x 2048 bfloat16 in 102 us with 8, 126
 //   with 4, 195 with 16 (146 registers: one block a compute unit, its loads no longer ahead of its arithmetic).
 // - From REC_MANY_TILES tiles on a strand is 64 lanes wide, 256 bytes of a position: 32 x 2048 x 4096 bfloat16 330 against 367 us.
-// - Below REC_FEW_TILES tiles of 32 lanes, records of REC_LEAST_LINKS links or more are cut into chains: 1 x 4096 x 512 bfloat16
-//   14 against 49 us, 4 x 2048 x 1024 19 against 32, 6 x 2048 x 2048 (192 tiles) 40 against 46, at 256 tiles 109 against 102;
+// - Below REC_FEW_TILES tiles of 32 lanes, records of REC_LEAST_LINKS links or more are cut into chains (the zeroing of their granules
+//   counted): 1 x 4096 x 512 bfloat16 13 against 49 us, 4 x 2048 x 1024 18 against 32, 6 x 2048 x 2048 (192 tiles) 40 against 46, at 256 tiles 109 against 102;
 //   three links (1 x 600 x 512) 11.2 against 10.5, their gradients 15.3 against 17.6.  Gradients, with five tensors on their
 //   way, gain up to REC_FEW_TILES_BACKWARD tiles: 4 x 8192 x 4096 (256 tiles) 301 against 334, 8 x 2048 x 2500 (320) 114
-//   against 159.
-// - Fewer than REC_FEW_ROWS rows of REC_LEAST_ROW_LINKS links or more are cut into links: 1 x 65536 float32 7.9 against 18.1 us (the
-//   granules' 2 us included), 64 x 32768 13.1 against 13.3, its gradients 15.7 against 18.5; 200 x 32768 23.7 against 16.7.
+//   against 159, both without the byte an element that `fine` adds (321 and 125 with it).
+// - Fewer than REC_FEW_ROWS rows of REC_LEAST_ROW_LINKS links or more are cut into links: 1 x 65536 float32 7.3 against 18.1 us (the
+//   granules' 1.4 us included), 64 x 32768 12.7 against 13.3, its gradients 15.4 against 18.5; 200 x 32768 23.7 against 17.
 constexpr int REC_LENGTH = 8;
 constexpr long long REC_MANY_TILES = 512, REC_FEW_TILES = 256, REC_FEW_TILES_BACKWARD = 512, REC_LEAST_LINKS = 3;
 constexpr long long REC_FEW_ROWS = 128, REC_LEAST_ROW_LINKS = 3;
@@ -246,11 +246,11 @@ template <typename T, int THREADS, int NP, int MODE> static void launch_row(cons
 
 template <typename T, int MODE> static void launch_distill(const DistillArgs &q, float c, hipStream_t st)
 {
-    // Groups of lanes up to 64 actions (40000 x 64 float32, 20 entries, loss and gradient: 20 us, a block a row 82; at 200 actions
-    // groups of a whole wave took 125, the block 55).  Then as few waves a row as keep its packs in registers: 6000 bfloat16 in 78 us
-    // with 128 threads of 8 packs, 89 with 64 of 16; 32000 in 118 with 256 of 16, 131 with 512 of 8, 165 with 1024 of 4, 141 read
-    // twice; 1000 float32 in 38 with 4 packs a thread, 45 with 8 (idle packs cost exponentials).  Wider rows are read twice:
-    // 131071 in 165, 183 where 1024 threads hold 17 packs each; their loss alone in 76 with 512 threads, 88 with 1024, their gradient
+    // Groups of lanes up to 64 actions (40000 x 64 float32, 20 entries, loss and gradient: 21 us, a block a row 82; at 200 actions
+    // groups of a whole wave took 125, the block 57).  Then as few waves a row as keep its packs in registers: 12000 x 6000 bfloat16
+    // in 79 us with 128 threads of 8 packs, 89 with 64 of 16; 4096 x 32000 in 118 with 256 of 16, 131 with 512 of 8, 165 with 1024 of
+    // 4, 141 read twice; 20000 x 1000 float32 in 37 with 4 packs a thread, 45 with 8 (idle packs cost exponentials).  Wider rows are
+    // read twice: 1023 x 131071 in 165, 183 where 1024 threads hold 17 packs each; their loss alone in 76 with 512 threads, 88 with 1024, their gradient
     // alone in 106 with 1024, 117 with 512.
     constexpr int W = 16 / (int)sizeof(T);   // actions of a pack
     const int packs = (q.V + W - 1) / W + 1;   // one more where a row begins inside a pack

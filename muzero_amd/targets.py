@@ -113,7 +113,8 @@ def linear_recurrence(gate: torch.Tensor, x: torch.Tensor, state: Optional[torch
     first position, float32 (float64 with float64 tensors) - zeros if None.  Returns (y, state behind the last position);
     that state continues the recurrence in a later call, one position at a time if need be.  Arithmetic is float32 (float64
     for float64), each y rounded once.  The products of the gates over a record must not overflow, which |gate| <= 1
-    ensures; a gate of 0 cuts the record."""
+    ensures; a gate of 0 cuts the record; what follows an infinite y of its row is infinite or NaN.  Where a 16-bit gate requires a
+    gradient, a byte an element is kept beside y for it.  Differentiable once and backward only; a trace or a tangent raises."""
     if not (torch.is_tensor(gate) and torch.is_tensor(x) and gate.is_cuda and x.is_cuda):
         raise _engine.EngineError('linear_recurrence needs device tensors (there is no CPU fallback)')
     shape, dtype = x.shape, x.dtype

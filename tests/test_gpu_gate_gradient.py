@@ -20,7 +20,8 @@ def laid_out(t, layout):
 
 
 @pytest.mark.parametrize('dtype', [torch.bfloat16, torch.float16])
-@pytest.mark.parametrize('shape,layout', [((64, 1, 136), 'channels'), ((5, 7, 33), 'channels'), ((8, 200, 66), 'channels'),
+@pytest.mark.parametrize('shape,layout', [((64, 1, 136), 'channels'), ((6, 6, 136), 'channels'), ((3, 8, 64), 'channels'),
+                                          ((5, 7, 33), 'channels'), ((1, 1501, 33), 'channels'), ((8, 200, 66), 'channels'),
                                           ((3, 300, 65), 'channels'), ((1, 1500, 130), 'channels'), ((2, 2049, 40), 'channels'),
                                           ((40, 300, 1), 'channels'), ((3, 77, 6), 'time'), ((4, 1000, 5), 'time'),
                                           ((1, 24577, 3), 'time'), ((33, 50, 1), 'sequences'), ((7, 1, 1), 'sequences')])
@@ -58,3 +59,34 @@ def test_values_at_the_ends_of_the_types():
     y, _ = linear_recurrence(gate, torch.full((1, 3, 1), 60000.0, dtype=torch.float16, device='cuda'))
     da, = torch.autograd.grad(y, gate, torch.full_like(y, 0.25))
     assert y[0, 1:].isinf().all() and da[0, 2].isinf().all() and da[0, 1, 0] == 30000.0
+
+
+@pytest.mark.parametrize('shape', [(3, 300, 66), (1, 1500, 66), (9, 5, 8), (5, 600, 1)])
+def test_a_captured_training_step(shape):
+    """What the forward pass keeps for the gate's gradient is the captured pass's own, on every replay."""
+    from muzero_amd.targets import linear_recurrence
+    a, x, s = inputs(*shape, torch.bfloat16)
+    dy = torch.randn(shape, generator=torch.Generator().manual_seed(3)).bfloat16().cuda()
+
+    def step(gate, x):
+        y, last = linear_recurrence(gate, x, s)
+        return (y, last) + torch.autograd.grad((y, last), (gate, x), (dy, s))
+
+    leaves = lambda k: (a.clone().requires_grad_(), (x * k).requires_grad_())  # noqa: E731
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(*leaves(1))
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    g, z = leaves(1)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step(g, z)
+    for k in range(1, 5):
+        with torch.no_grad():
+            z.copy_(x * k)
+        graph.replay()
+        want = step(*leaves(k))
+        torch.cuda.synchronize()
+        assert all(torch.equal(p, q) for p, q in zip(out, want))
