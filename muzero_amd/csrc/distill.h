@@ -125,7 +125,8 @@ __device__ __forceinline__ double divergence(const DistillArgs &q, const Mass &e
     const double ratio = e.rest == 0 ? 1.0 : e.rest * dsum / dtail;
     const double l = log(lane == 1 ? dsum : lane == 2 && !(e.rest == 0) ? ratio : lane == 0 && e.norm > 0 ? e.norm : 1.0);
     const double of_sum = __shfl(l, 1, G), of_ratio = __shfl(l, 2, G);
-    return e.ent - e.mass * l - (cross - e.mass * of_sum) + (e.rest == 0 ? 0.0 : e.rest * (of_ratio + (mt == m ? 0.0 : ((double)m - (double)mt) * q.inv_tau)));
+    const double below = mt == m ? 0.0 : ((double)m - (double)mt) * q.inv_tau;
+    return e.ent - e.mass * l - (cross - e.mass * of_sum) + (e.rest == 0 ? 0.0 : e.rest * (of_ratio + below));
 }
 
 // Small action sets: G lanes of a wave hold a row, E actions and 4 entries a lane, all of it in registers.  MODE 0: loss and

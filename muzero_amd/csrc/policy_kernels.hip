@@ -29,7 +29,8 @@ static size_t size_of(int type) { return type == MZ_F64 ? 8 : type == MZ_F32 ? 4
 //   with 4, 195 with 16 (146 registers: one block a compute unit, its loads no longer ahead of its arithmetic).
 // - From REC_MANY_TILES tiles on a strand is 64 lanes wide, 256 bytes of a position: 32 x 2048 x 4096 bfloat16 330 against 367 us.
 // - Below REC_FEW_TILES tiles of 32 lanes, records of REC_LEAST_LINKS links or more are cut into chains (the zeroing of their granules
-//   counted): 1 x 4096 x 512 bfloat16 13 against 49 us, 4 x 2048 x 1024 18 against 32, 6 x 2048 x 2048 (192 tiles) 40 against 46, at 256 tiles 109 against 102;
+//   counted): 1 x 4096 x 512 bfloat16 13 against 49 us, 4 x 2048 x 1024 18 against 32, 6 x 2048 x 2048 (192 tiles) 40 against 46, at
+//   256 tiles 109 against 102;
 //   three links (1 x 600 x 512) 11.2 against 10.5, their gradients 15.3 against 17.6.  Gradients, with five tensors on their
 //   way, gain up to REC_FEW_TILES_BACKWARD tiles: 4 x 8192 x 4096 (256 tiles) 301 against 334, 8 x 2048 x 2500 (320) 114
 //   against 159, both without the byte an element that `fine` adds (321 and 125 with it).
@@ -176,7 +177,8 @@ static int check_recurrence(const mz_recurrence *a, bool backward, const char *f
     if (!a->gate.p || !a->x.p || !a->out.p) return api_fail(MZ_ERR_ARG, std::string(fn) + ": null tensor");
     if (backward && (a->out_gate.p != nullptr) != (a->y.p != nullptr))
         return api_fail(MZ_ERR_ARG, std::string(fn) + ": the gates' gradient needs the outputs, and nothing else does");
-    if (size_of(a->type) == 2 && a->fine.p && ((uintptr_t)a->fine.p | (uint64_t)a->fine.stride_b | (uint64_t)a->fine.stride_t | (uint64_t)a->fine.stride_d) % 4 != 0)
+    const mz_strided &f = a->fine;
+    if (size_of(a->type) == 2 && f.p && ((uintptr_t)f.p | (uint64_t)f.stride_b | (uint64_t)f.stride_t | (uint64_t)f.stride_d) % 4 != 0)
         return api_fail(MZ_ERR_ARG, std::string(fn) + ": fine and its strides must be multiples of 4 bytes");
     return MZ_OK;
 }

@@ -164,10 +164,10 @@ template <typename T, int G> __global__ __launch_bounds__(256) void k_verify_gro
 
 // Wide action sets: one block per sequence.  The row is cut into stretches of two wide loads of a wave; a wave sums whole
 // stretches, the first wave finds the stretch in which the running sum passes the goal and walks that one again.
-// 256 x 100003 float32: 35 us (205 MB, 5.9 TB/s with part of the rows in cache); 2000 x 32000 bfloat16 100 us (256 MB;
-// waves wait for three quarters of their cycles and the vector units issue in a tenth of theirs: a stretch's sixteen dependent
-// float64 additions and its fold stand between a wave's loads); one sequence of 32000 float32: 10 us, of which the launch is 3 and four dependent trips to memory most of
-// the rest; one of 130000: 24 us, what one compute unit can read.
+// 256 x 100003 float32: 34 us (205 MB, 6 TB/s with part of the rows in cache); 2000 x 32000 bfloat16 100 us (256 MB; waves wait for
+// three quarters of their cycles and the vector units issue in a tenth of theirs: a stretch's sixteen dependent float64 additions
+// and its fold stand between a wave's loads); one sequence of 32000 float32: 10 us, of which the launch is 3 and four dependent trips
+// to memory most of the rest; one of 130000: 25 us, what one compute unit can read.
 constexpr int STRETCH_LOADS = 2;
 template <typename T> constexpr int STRETCH = STRETCH_LOADS * 64 * (16 / (int)sizeof(T));
 
